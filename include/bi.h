@@ -311,6 +311,79 @@ int bi_rope_kv(const void* qkv, int64_t B, int64_t L, int64_t hq, int64_t hk, in
  * rounded to the storage type before the product, as silu(g) * u in two steps. */
 int bi_swiglu(const void* gu, void* out, int64_t M, int64_t I, int dtype, void* stream);
 
+/*
+ * ---------------------------------------------------------------------------
+ * A serving step over a KV cache in pages.  No reference counterpart (its cache is one
+ * contiguous array per batch).  A page holds page_size consecutive tokens of one request as
+ * (Hkv, page_size, D); a request's block table row lists its pages in order; a slot is
+ * page * page_size + place in the page.
+ * ---------------------------------------------------------------------------
+ */
+
+/* The step's token layout from the request lengths, in one launch:
+ *   query_lens, context_lens  (R,) new tokens and tokens already cached of each request;
+ *   query_start (R + 1,) <- sums of query_lens;  seq_lens (R,) <- context + query;
+ *   positions, slots (T,) <- of each new token, request after request; -1 behind the last.
+ *   block_table (R, width), row stride table_stride: columns below ceil(context / page_size)
+ *          are read; where free_pages is given, the columns that the new tokens need beyond
+ *          those are filled with free_pages[*free_head ...] in request order and
+ *          *next_head <- the place behind the last page taken.  next_head must not be
+ *          free_head.  With free_pages == NULL the table must hold every page already.
+ * Lengths that are negative or do not fit the table (the request then brings no tokens), more
+ * tokens than T, and tokens without a page (slot -1, and -1 in the table where the free pages
+ * ran out) record site 1, reason 2 (tagged bit 19) in the device error word. */
+int bi_paged_plan(const int32_t* query_lens, const int32_t* context_lens, int64_t R, int64_t T,
+                  int32_t* block_table, int64_t table_stride, int64_t width, int64_t page_size,
+                  const int32_t* free_pages, int64_t n_free, const int32_t* free_head,
+                  int32_t* query_start, int32_t* seq_lens, int64_t* positions, int64_t* slots,
+                  int32_t* next_head, void* stream);
+
+/* bi_rope_kv over pages: qkv (T, (hq + 2 hk) * hd) with row stride qkv_stride; token t sits at
+ * positions[t] and its rotated k and its v go to slots[t] of k_cache / v_cache (n_pages, hk,
+ * page_size, hd), strides of page, head and token (the last dim contiguous); the rotated q to
+ * q_out (T, hq, hd).  The first `rot` elements of a head are rotated (halves of rot / 2;
+ * tables (n_pos, rot / 2)), the others copied.  A token with positions[t] < 0 is padding and
+ * touches nothing; slots[t] < 0 writes no k and v.  Positions and slots past the tables or
+ * the caches write nothing and record site 2, reason 2 (bit 19) in the device error word.
+ * Slots must differ: of tokens with the same slot an unspecified mixture remains. */
+int bi_rope_kv_paged(const void* qkv, int64_t qkv_stride, int64_t T, int64_t hq, int64_t hk,
+                     int64_t hd, int64_t rot, const float* cos_tab, const float* sin_tab,
+                     int64_t n_pos, const int64_t* positions, const int64_t* slots, void* q_out,
+                     void* k_cache, const int64_t k_strides[3], void* v_cache,
+                     const int64_t v_strides[3], int64_t n_pages, int64_t page_size, int dtype,
+                     void* stream);
+
+/* Bytes of workspace that bi_paged_sdpa makes full use of (of T = 0: the least it takes;
+ * with less than the full amount long requests are split over fewer blocks, same bits). */
+int64_t bi_paged_sdpa_workspace(int64_t T, int64_t R, int64_t H, int64_t D, int64_t width,
+                                int64_t page_size);
+
+/*
+ * Attention of each request's new tokens over its sequence in the pages:
+ *   out[t, h, :] = sum_i softmax_i(scale * q[t, h, :] . k_i) v_i
+ * over the keys i <= p of the token's request, p = seq_lens[r] - (query_start[r + 1] -
+ * query_start[r]) + (t - query_start[r]); with window > 0 only those with i > p - window or
+ * i < first_tokens.  The new tokens' keys and values are in the cache already.
+ *   q, out  (T, H, D), element strides of token and head, the last dim contiguous; rows of
+ *           `out` outside every request are left as they were.
+ *   k, v    (n_pages, Hkv, page_size, D), strides of page, head and token.
+ *   sinks   nullable (H,) in the q dtype: one extra logit per head.
+ * H % Hkv == 0; D a multiple of 32 up to 256; scale finite and >= 0.  A row that sees no key
+ * returns zeros.  Keys that a row does not see do not reach it, whatever they hold.  A page
+ * number outside [0, n_pages) reads as zeros.  query_start and seq_lens are clamped to T and
+ * to what a row of the table holds.
+ * Invariance: a row's bits depend on its q, its keys and values, (dtype, D, H / Hkv,
+ * page_size), scale, window, first_tokens and sinks alone -- not on the batch, on how many
+ * tokens arrive together, on which pages hold the sequence or on the workspace's size. */
+int bi_paged_sdpa(const void* q, const int64_t q_strides[2], const void* k,
+                  const int64_t k_strides[3], const void* v, const int64_t v_strides[3],
+                  int64_t n_pages, int64_t page_size, const int32_t* block_table,
+                  int64_t table_stride, int64_t width, const int32_t* query_start,
+                  const int32_t* seq_lens, const void* sinks, float scale, int64_t window,
+                  int64_t first_tokens, int64_t T, int64_t R, int64_t H, int64_t Hkv, int64_t D,
+                  int dtype, void* out, const int64_t out_strides[2], void* workspace,
+                  int64_t workspace_bytes, void* stream);
+
 /* Static description of a status code. */
 const char* bi_status_string(int status);
 

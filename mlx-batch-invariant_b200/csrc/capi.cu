@@ -1,6 +1,6 @@
 // extern "C" entry points of libbi.so (declared in include/bi.h): argument
 // validation, route selection and error reporting.  The kernels live in
-// gemm_tcgen05.cu, gemm_simt.cu and sdpa.cu.
+// gemm_tcgen05.cu, gemm_simt.cu, sdpa.cu, harness.cu, paged.cu and paged_sdpa.cu.
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -576,6 +576,179 @@ int bi_swiglu(const void* gu, void* out, int64_t M, int64_t I, int dtype, void* 
   return launch_swiglu(gu, out, M, I, dtype, static_cast<cudaStream_t>(stream));
 }
 
+int bi_paged_plan(const int32_t* query_lens, const int32_t* context_lens, int64_t R, int64_t T,
+                  int32_t* block_table, int64_t table_stride, int64_t width, int64_t page_size,
+                  const int32_t* free_pages, int64_t n_free, const int32_t* free_head,
+                  int32_t* query_start, int32_t* seq_lens, int64_t* positions, int64_t* slots,
+                  int32_t* next_head, void* stream) {
+  g_msg[0] = '\0';
+  if (R < 0 || T < 0 || width < 0 || page_size <= 0 || n_free < 0) {
+    return set_error(BI_ERR_INVALID, "negative size, or page_size below 1");
+  }
+  if (R >= INT32_MAX || T >= INT32_MAX || width > INT32_MAX || page_size > INT32_MAX ||
+      n_free > INT32_MAX) {
+    return set_error(BI_ERR_UNSUPPORTED, "sizes of 2^31 and above are not supported");
+  }
+  if (query_start == nullptr ||
+      (R > 0 && (query_lens == nullptr || context_lens == nullptr || seq_lens == nullptr ||
+                 (width > 0 && block_table == nullptr))) ||
+      (T > 0 && (positions == nullptr || slots == nullptr)) ||
+      (free_pages != nullptr && (free_head == nullptr || next_head == nullptr))) {
+    return set_error(BI_ERR_INVALID, "null pointer");
+  }
+  if (R > 1 && table_stride < width) {
+    return set_error(BI_ERR_INVALID, "the block table's row stride is smaller than its row");
+  }
+  int st = check_device();
+  if (st) return st;
+  PlanArgs a{query_lens, context_lens, R, T, block_table, table_stride, width, page_size,
+             free_pages, n_free, free_head, query_start, seq_lens, positions, slots, next_head};
+  return launch_paged_plan(a, static_cast<cudaStream_t>(stream));
+}
+
+int bi_rope_kv_paged(const void* qkv, int64_t qkv_stride, int64_t T, int64_t hq, int64_t hk,
+                     int64_t hd, int64_t rot, const float* cos_tab, const float* sin_tab,
+                     int64_t n_pos, const int64_t* positions, const int64_t* slots, void* q_out,
+                     void* k_cache, const int64_t k_strides[3], void* v_cache,
+                     const int64_t v_strides[3], int64_t n_pages, int64_t page_size, int dtype,
+                     void* stream) {
+  g_msg[0] = '\0';
+  if (dtype != BI_F32 && dtype != BI_F16 && dtype != BI_BF16) {
+    return set_error(BI_ERR_INVALID, "unknown dtype %d", dtype);
+  }
+  if (T < 0 || hq < 0 || hk < 0 || hd <= 0 || hd % 2 != 0 || rot < 0 || rot % 2 != 0 || rot > hd ||
+      n_pos < 0 || n_pages < 0 || page_size <= 0) {
+    return set_error(BI_ERR_INVALID, "bad sizes (hd and rot must be even, 0 <= rot <= hd)");
+  }
+  if (T >= INT32_MAX || (hq + 2 * hk) * hd >= INT32_MAX) {
+    return set_error(BI_ERR_UNSUPPORTED, "sizes of 2^31 and above are not supported");
+  }
+  if (qkv_stride < (hq + 2 * hk) * hd && T > 1) {
+    return set_error(BI_ERR_INVALID, "row stride of qkv smaller than the row");
+  }
+  if (T > 0 && (qkv == nullptr || positions == nullptr || slots == nullptr ||
+                (rot > 0 && (cos_tab == nullptr || sin_tab == nullptr)) ||
+                (hq > 0 && q_out == nullptr) ||
+                (hk > 0 && (k_cache == nullptr || v_cache == nullptr || k_strides == nullptr ||
+                            v_strides == nullptr)))) {
+    return set_error(BI_ERR_INVALID, "null pointer");
+  }
+  int st = check_device();
+  if (st) return st;
+  RopePagedArgs a{qkv, qkv_stride, T, hq, hk, hd, rot, cos_tab, sin_tab, n_pos, positions, slots,
+                  q_out, k_cache, v_cache, {0, 0, 0}, {0, 0, 0}, n_pages, page_size};
+  for (int i = 0; i < 3 && hk > 0 && T > 0; ++i) {
+    a.ks[i] = k_strides[i];
+    a.vs[i] = v_strides[i];
+  }
+  return launch_rope_paged(a, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int64_t bi_paged_sdpa_workspace(int64_t T, int64_t R, int64_t H, int64_t D, int64_t width,
+                                int64_t page_size) {
+  if (T < 0 || R < 0 || H < 0 || D < 0 || width < 0 || page_size < 0) return 0;
+  return paged_sdpa_workspace(T, R, H, D, width, page_size);
+}
+
+int bi_paged_sdpa(const void* q, const int64_t q_strides[2], const void* k,
+                  const int64_t k_strides[3], const void* v, const int64_t v_strides[3],
+                  int64_t n_pages, int64_t page_size, const int32_t* block_table,
+                  int64_t table_stride, int64_t width, const int32_t* query_start,
+                  const int32_t* seq_lens, const void* sinks, float scale, int64_t window,
+                  int64_t first_tokens, int64_t T, int64_t R, int64_t H, int64_t Hkv, int64_t D,
+                  int dtype, void* out, const int64_t out_strides[2], void* workspace,
+                  int64_t workspace_bytes, void* stream) {
+  g_msg[0] = '\0';
+  if (dtype != BI_F32 && dtype != BI_F16 && dtype != BI_BF16) {
+    return set_error(BI_ERR_INVALID, "unknown dtype %d", dtype);
+  }
+  if (T < 0 || R < 0 || H < 0 || Hkv < 0 || D <= 0 || n_pages < 0 || page_size <= 0 || width < 0 ||
+      window < 0 || first_tokens < 0) {
+    return set_error(BI_ERR_INVALID, "negative or empty dimension");
+  }
+  if (Hkv == 0 || H % Hkv != 0) return set_error(BI_ERR_INVALID, "H must be a multiple of Hkv");
+  if (D % 32 != 0) return set_error(BI_ERR_INVALID, "the head dimension must be a multiple of 32");
+  if (D > 256) {
+    return set_error(BI_ERR_UNSUPPORTED, "head dim %lld is not built (at most 256)",
+                     static_cast<long long>(D));
+  }
+  if (!(scale >= 0.f) || scale > 3.0e38f) {
+    return set_error(BI_ERR_INVALID, "scale must be finite and not negative");
+  }
+  if (first_tokens > 0 && window == 0) {
+    return set_error(BI_ERR_INVALID, "first_tokens needs a window");
+  }
+  if (T == 0 || R == 0 || H == 0) return BI_OK;
+  if (T >= INT32_MAX || R >= INT32_MAX || H >= INT32_MAX || n_pages >= INT32_MAX ||
+      page_size >= INT32_MAX || width >= INT32_MAX) {
+    return set_error(BI_ERR_UNSUPPORTED, "sizes of 2^31 and above are not supported");
+  }
+  if (q == nullptr || out == nullptr || query_start == nullptr || seq_lens == nullptr ||
+      q_strides == nullptr || out_strides == nullptr || k_strides == nullptr ||
+      v_strides == nullptr || (width > 0 && block_table == nullptr) ||
+      (n_pages > 0 && (k == nullptr || v == nullptr))) {
+    return set_error(BI_ERR_INVALID, "null pointer");
+  }
+  if (width == 0 || n_pages == 0) {
+    return set_error(BI_ERR_INVALID, "the block table and the cache must not be empty");
+  }
+  if (R > 1 && table_stride < width) {
+    return set_error(BI_ERR_INVALID, "the block table's row stride is smaller than its row");
+  }
+  const int64_t vec = 16 / elem_size(dtype);
+  bool ok = aligned16(q) && aligned16(k) && aligned16(v) && q_strides[0] % vec == 0 &&
+            q_strides[1] % vec == 0;
+  for (int i = 0; i < 3; ++i) {
+    ok = ok && k_strides[i] > 0 && v_strides[i] > 0 && k_strides[i] % vec == 0 &&
+         v_strides[i] % vec == 0;
+  }
+  ok = ok && q_strides[0] > 0 && q_strides[1] > 0;
+  if (!ok) {
+    return set_error(BI_ERR_MISALIGNED, "q and the caches must be 16-byte aligned with positive "
+                     "strides that are multiples of 16 bytes");
+  }
+  if (workspace == nullptr || !aligned16(workspace) ||
+      workspace_bytes < paged_sdpa_workspace(0, R, H, D, width, page_size)) {
+    return set_error(BI_ERR_INVALID, "workspace is null, misaligned or smaller than "
+                     "bi_paged_sdpa_workspace of no tokens");
+  }
+  int st = check_device();
+  if (st) return st;
+  PagedSdpaArgs a;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  for (int i = 0; i < 2; ++i) {
+    a.qs[i] = q_strides[i];
+    a.os[i] = out_strides[i];
+  }
+  for (int i = 0; i < 3; ++i) {
+    a.ks[i] = k_strides[i];
+    a.vs[i] = v_strides[i];
+  }
+  a.table = block_table;
+  a.table_stride = table_stride;
+  a.width = width;
+  a.query_start = query_start;
+  a.seq_lens = seq_lens;
+  a.sinks = sinks;
+  a.scale = scale;
+  a.window = window;
+  a.first = first_tokens;
+  a.T = T;
+  a.R = R;
+  a.H = H;
+  a.Hkv = Hkv;
+  a.D = D;
+  a.n_pages = n_pages;
+  a.page = page_size;
+  a.out = out;
+  a.dtype = dtype;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
+  return launch_paged_sdpa(a, static_cast<cudaStream_t>(stream));
+}
+
 const char* bi_status_string(int status) {
   switch (status) {
     case BI_OK: return "ok";
@@ -598,9 +771,11 @@ int bi_device_error(int clear) {
   const unsigned s = read_error_sdpa(clear != 0);
   const unsigned h = read_error_harness(clear != 0);
   const unsigned t = read_error_tf32x3(clear != 0);
+  const unsigned pg = read_error_paged(clear != 0);
   if (w == 0 && s != 0) w = s | (1u << 16);  // sdpa sites are tagged in bit 16
   if (w == 0 && h != 0) w = h | (1u << 17);  // decoder-harness sites in bit 17
   if (w == 0 && t != 0) w = t | (1u << 18);  // fp32 tensor-core GEMM sites in bit 18
+  if (w == 0 && pg != 0) w = pg | (1u << 19);  // plan and rotary write over pages in bit 19
   return static_cast<int>(w);
 }
 

@@ -101,6 +101,64 @@ int launch_rope_kv(const RopeArgs& a, int dtype, cudaStream_t stream);
 int launch_swiglu(const void* gu, void* out, int64_t M, int64_t I, int dtype,
                   cudaStream_t stream);
 
+// The serving step over a KV cache in pages (paged.cu, paged_sdpa.cu).
+struct PlanArgs {
+  const int* query_lens;    // (R,) new tokens
+  const int* context_lens;  // (R,) tokens already cached
+  int64_t R, T;             // requests; tokens the two token arrays hold
+  int* table;               // (R, width) pages, row stride table_stride
+  int64_t table_stride, width, page;
+  const int* free_pages;    // nullable: the tables are complete
+  int64_t n_free;
+  const int* free_head;     // (1,) first free page's place in free_pages
+  int* query_start;         // (R + 1,)
+  int* seq_lens;            // (R,)
+  int64_t* positions;       // (T,), -1 behind the last token
+  int64_t* slots;           // (T,), likewise
+  int* next_head;           // (1,)
+};
+int launch_paged_plan(const PlanArgs& a, cudaStream_t stream);
+
+struct RopePagedArgs {
+  const void* qkv;          // (T, (hq + 2 hk) * hd), row stride qkv_stride
+  int64_t qkv_stride, T, hq, hk, hd, rot;
+  const float* cos_tab;     // (n_pos, rot / 2)
+  const float* sin_tab;
+  int64_t n_pos;
+  const int64_t* positions;  // (T,)
+  const int64_t* slots;      // (T,)
+  void* q_out;               // (T, hq, hd)
+  void* k_cache;             // (n_pages, hk, page, hd), strides ks of page, head, token
+  void* v_cache;
+  int64_t ks[3], vs[3], n_pages, page;
+};
+int launch_rope_paged(const RopePagedArgs& a, int dtype, cudaStream_t stream);
+
+struct PagedSdpaArgs {
+  const void* q;             // (T, H, D), strides qs of token, head
+  int64_t qs[2];
+  const void* k;             // (n_pages, Hkv, page, D), strides ks of page, head, token
+  const void* v;
+  int64_t ks[3], vs[3];
+  const int* table;          // (R, width), row stride table_stride
+  int64_t table_stride, width;
+  const int* query_start;    // (R + 1,)
+  const int* seq_lens;       // (R,)
+  const void* sinks;         // nullable (H,)
+  float scale;
+  int64_t window;            // 0: none
+  int64_t first;             // first tokens that stay visible
+  int64_t T, R, H, Hkv, D, n_pages, page;
+  void* out;                 // (T, H, D), strides os
+  int64_t os[2];
+  int dtype;
+  void* workspace;
+  int64_t workspace_bytes;
+};
+int64_t paged_sdpa_workspace(int64_t T, int64_t R, int64_t H, int64_t D, int64_t width,
+                             int64_t page);
+int launch_paged_sdpa(const PagedSdpaArgs& a, cudaStream_t stream);
+
 int launch_gemm_tc(const GemmArgs& g, cudaStream_t stream);
 // g.out points at column cols[rank] of the output whose first column is out_base.
 // unpack = false leaves the peers' blocks in this rank's staging area (launch
@@ -120,6 +178,7 @@ unsigned read_error_gemm_tc(bool clear);
 unsigned read_error_sdpa(bool clear);
 unsigned read_error_harness(bool clear);
 unsigned read_error_tf32x3(bool clear);
+unsigned read_error_paged(bool clear);
 
 // Per-thread message for bi_last_error().
 int set_error(int status, const char* fmt, ...);

@@ -20,11 +20,12 @@ import math
 import torch
 import torch.nn.functional as F
 
-from . import _ops  # noqa: F401  (registers mlx_bi::gemm and mlx_bi::sdpa)
+from . import _ops  # noqa: F401  (registers the mlx_bi:: ops)
 from ._attention import _mask_args, _sdpa, scaled_dot_product_attention
 from ._attention import head_dims_built
 from ._gemm import QUANT_BITS, SIMT_TILE, TILE, addmm, linear, matmul, quantized_linear, tile_for
 from ._gemm import float32_gemm, get_float32_gemm, set_float32_gemm
+from ._paged import PagedPlan, paged_attention, paged_plan, rope_kv_paged
 
 __all__ = [
     "quantized_linear",
@@ -33,6 +34,10 @@ __all__ = [
     "addmm",
     "linear",
     "scaled_dot_product_attention",
+    "paged_plan",
+    "PagedPlan",
+    "rope_kv_paged",
+    "paged_attention",
     "batch_invariant_mode",
     "is_enabled",
     "TILE",

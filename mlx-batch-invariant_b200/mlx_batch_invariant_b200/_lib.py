@@ -91,6 +91,26 @@ def _bind(lib):
                                _vp, _vp, _vp, _i64_3, ctypes.c_int, _vp]
     lib.bi_swiglu.restype = ctypes.c_int
     lib.bi_swiglu.argtypes = [_vp, _vp, _i64, _i64, ctypes.c_int, _vp]
+    # (query_lens, context_lens, R, T, table, stride, width, page, free_pages, n_free,
+    #  free_head, query_start, seq_lens, positions, slots, next_head, stream)
+    lib.bi_paged_plan.restype = ctypes.c_int
+    lib.bi_paged_plan.argtypes = [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp,
+                                  _vp, _vp, _vp, _vp, _vp, _vp]
+    # (qkv, stride, T, hq, hk, hd, rot, cos, sin, n_pos, positions, slots, q, k_cache,
+    #  k_strides, v_cache, v_strides, n_pages, page, dtype, stream)
+    lib.bi_rope_kv_paged.restype = ctypes.c_int
+    lib.bi_rope_kv_paged.argtypes = [_vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64,
+                                     _vp, _vp, _vp, _vp, _i64_3, _vp, _i64_3, _i64, _i64,
+                                     ctypes.c_int, _vp]
+    lib.bi_paged_sdpa_workspace.restype = _i64
+    lib.bi_paged_sdpa_workspace.argtypes = [_i64] * 6
+    # (q, q_strides, k, k_strides, v, v_strides, n_pages, page, table, stride, width,
+    #  query_start, seq_lens, sinks, scale, window, first, T, R, H, Hkv, D, dtype, out,
+    #  out_strides, workspace, workspace_bytes, stream)
+    lib.bi_paged_sdpa.restype = ctypes.c_int
+    lib.bi_paged_sdpa.argtypes = [_vp, _i64_2, _vp, _i64_3, _vp, _i64_3, _i64, _i64, _vp, _i64,
+                                  _i64, _vp, _vp, _vp, ctypes.c_float, _i64, _i64, _i64, _i64,
+                                  _i64, _i64, _i64, ctypes.c_int, _vp, _i64_2, _vp, _i64, _vp]
 
 
 def lib():
