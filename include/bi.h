@@ -374,7 +374,10 @@ int64_t bi_paged_sdpa_workspace(int64_t T, int64_t R, int64_t H, int64_t D, int6
  * to what a row of the table holds.
  * Invariance: a row's bits depend on its q, its keys and values, (dtype, D, H / Hkv,
  * page_size), scale, window, first_tokens and sinks alone -- not on the batch, on how many
- * tokens arrive together, on which pages hold the sequence or on the workspace's size. */
+ * tokens arrive together, on which pages hold the sequence or on the workspace's size.  fp16 /
+ * bf16 with D = 64 or 128, H / Hkv <= 128 and a page_size that divides 128 (8 and up) or is a
+ * multiple of it run on the tensor cores with the weights rounded to the 16-bit type; else on
+ * the CUDA cores in fp32. */
 int bi_paged_sdpa(const void* q, const int64_t q_strides[2], const void* k,
                   const int64_t k_strides[3], const void* v, const int64_t v_strides[3],
                   int64_t n_pages, int64_t page_size, const int32_t* block_table,

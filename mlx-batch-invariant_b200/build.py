@@ -23,7 +23,7 @@ LIB = os.path.join(HERE, "mlx_batch_invariant_b200", "libbi.so")
 INCLUDE = os.path.join(ROOT, "include")
 
 SOURCES = ["capi.cu", "gemm_tcgen05.cu", "gemm_tf32x3.cu", "gemm_simt.cu", "sdpa.cu",
-           "harness.cu", "paged.cu", "paged_sdpa.cu"]
+           "harness.cu", "paged.cu", "paged_sdpa.cu", "paged_sdpa_tc.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
          "-I" + INCLUDE, "-I" + CSRC]

@@ -1,6 +1,7 @@
 // extern "C" entry points of libbi.so (declared in include/bi.h): argument
 // validation, route selection and error reporting.  The kernels live in
-// gemm_tcgen05.cu, gemm_simt.cu, sdpa.cu, harness.cu, paged.cu and paged_sdpa.cu.
+// gemm_tcgen05.cu, gemm_simt.cu, sdpa.cu, harness.cu, paged.cu, paged_sdpa.cu and
+// paged_sdpa_tc.cu.
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -772,10 +773,12 @@ int bi_device_error(int clear) {
   const unsigned h = read_error_harness(clear != 0);
   const unsigned t = read_error_tf32x3(clear != 0);
   const unsigned pg = read_error_paged(clear != 0);
+  const unsigned pa = read_error_paged_sdpa_tc(clear != 0);
   if (w == 0 && s != 0) w = s | (1u << 16);  // sdpa sites are tagged in bit 16
   if (w == 0 && h != 0) w = h | (1u << 17);  // decoder-harness sites in bit 17
   if (w == 0 && t != 0) w = t | (1u << 18);  // fp32 tensor-core GEMM sites in bit 18
   if (w == 0 && pg != 0) w = pg | (1u << 19);  // plan and rotary write over pages in bit 19
+  if (w == 0 && pa != 0) w = pa | (1u << 20);  // attention over pages in bit 20
   return static_cast<int>(w);
 }
 

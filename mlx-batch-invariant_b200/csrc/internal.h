@@ -101,7 +101,7 @@ int launch_rope_kv(const RopeArgs& a, int dtype, cudaStream_t stream);
 int launch_swiglu(const void* gu, void* out, int64_t M, int64_t I, int dtype,
                   cudaStream_t stream);
 
-// The serving step over a KV cache in pages (paged.cu, paged_sdpa.cu).
+// The serving step over a KV cache in pages (paged.cu, paged_sdpa.cu, paged_sdpa_tc.cu).
 struct PlanArgs {
   const int* query_lens;    // (R,) new tokens
   const int* context_lens;  // (R,) tokens already cached
@@ -179,6 +179,7 @@ unsigned read_error_sdpa(bool clear);
 unsigned read_error_harness(bool clear);
 unsigned read_error_tf32x3(bool clear);
 unsigned read_error_paged(bool clear);
+unsigned read_error_paged_sdpa_tc(bool clear);
 
 // Per-thread message for bi_last_error().
 int set_error(int status, const char* fmt, ...);

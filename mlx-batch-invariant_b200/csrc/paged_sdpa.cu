@@ -1,5 +1,5 @@
-// Attention of new tokens over a KV cache in pages (bi_paged_sdpa): the CUDA-core kernel, the
-// join of partial results and the host side.
+// Attention of new tokens over a KV cache in pages (bi_paged_sdpa): the CUDA-core route, the
+// join of partial results and the host side.  The tensor-core route is paged_sdpa_tc.cu.
 #include <algorithm>
 
 #include "paged_sdpa.cuh"
@@ -332,7 +332,8 @@ int64_t paged_sdpa_workspace(int64_t T, int64_t R, int64_t H, int64_t D, int64_t
 
 int launch_paged_sdpa(const PagedSdpaArgs& a, cudaStream_t stream) {
   using namespace psdpa;
-  const int rows = kSimtTile;
+  const bool tc = paged_tc_takes(a);
+  const int rows = tc ? 128 : kSimtTile;
   Params p;
   p.q = a.q;
   p.k = a.k;
@@ -366,7 +367,7 @@ int launch_paged_sdpa(const PagedSdpaArgs& a, cudaStream_t stream) {
   p.group_heads = std::min(p.G, rows);
   p.tile_tok = rows / p.group_heads;
   p.groups = p.Hkv * ((p.G + rows - 1) / rows);
-  p.target = 8 * device_sm_count();
+  p.target = (tc ? 2 : 8) * device_sm_count();
   p.fine_rows = 16;
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   p.any_split = reinterpret_cast<int*>(ws);
@@ -380,7 +381,8 @@ int launch_paged_sdpa(const PagedSdpaArgs& a, cudaStream_t stream) {
   const int64_t tiles = a.T / p.tile_tok + std::min(a.R, a.T);
   const int64_t items = tiles * p.groups + 4LL * p.target + 1;
   if (items > INT32_MAX) return set_error(BI_ERR_UNSUPPORTED, "too many query tiles");
-  const int st = dispatch(p, a.dtype, a.D, items, false, stream);
+  const int st = tc ? launch_paged_tc(a, p, items, stream)
+                    : dispatch(p, a.dtype, a.D, items, false, stream);
   if (st) return st;
   return dispatch(p, a.dtype, a.D, 0, true, stream);
 }

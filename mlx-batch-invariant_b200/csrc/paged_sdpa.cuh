@@ -281,4 +281,9 @@ __device__ __forceinline__ void grid_wait() {
 }
 
 }  // namespace psdpa
+
+// 16-bit tensor-core route (paged_sdpa_tc.cu); tiles of 128 rows.
+bool paged_tc_takes(const PagedSdpaArgs& a);
+int launch_paged_tc(const PagedSdpaArgs& a, const psdpa::Params& p, int64_t items,
+                    cudaStream_t stream);
 }  // namespace bi
