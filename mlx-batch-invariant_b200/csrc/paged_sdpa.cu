@@ -1,6 +1,7 @@
 // Attention of new tokens over a KV cache in pages (bi_paged_sdpa): the CUDA-core route, the
 // join of partial results and the host side.  The tensor-core route is paged_sdpa_tc.cu.
 #include <algorithm>
+#include <limits>
 
 #include "paged_sdpa.cuh"
 
@@ -352,7 +353,8 @@ int launch_paged_sdpa(const PagedSdpaArgs& a, cudaStream_t stream) {
   p.seq_lens = a.seq_lens;
   p.sinks = a.sinks;
   p.out = a.out;
-  p.scale_log2 = a.scale * kLog2e;
+  // (never 0: the score of a masked key is -inf, and -inf x 0 would be NaN)
+  p.scale_log2 = std::max(a.scale * kLog2e, std::numeric_limits<float>::min());
   p.window = a.window <= 0 || a.window >= INT32_MAX ? INT32_MAX : static_cast<int>(a.window);
   p.first = static_cast<int>(std::min<int64_t>(a.first, INT32_MAX));
   if (p.window == INT32_MAX) p.first = 0;

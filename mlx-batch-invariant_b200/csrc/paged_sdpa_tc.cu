@@ -30,7 +30,7 @@ constexpr int kThreads = 256;
 constexpr int kTile = 128;            // rows of a tile and keys of a step
 constexpr int kRegsSoftmax = 208;     // 128 x (208 + 48) = 256 x 128, the launch's registers
 constexpr int kRegsOther = 48;
-constexpr int kTmemCols = 256;        // S / P at 0, O at 128
+constexpr int kTmemCols = 256;        // S at 0 (P over its second half), O at 128
 constexpr float kSlack = 8.f;         // log 2 of how far weights may exceed 1
 
 enum : unsigned { kSiteProducer = 1, kSiteMma = 2, kSiteSoftmax = 3, kSiteDrain = 4 };
@@ -58,13 +58,25 @@ __device__ __forceinline__ void tmem_ld_x1(uint32_t taddr, uint32_t& r) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr)
                : "memory");
 }
-__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_ld_x64(uint32_t taddr, uint32_t (&r)[64]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-      "r"(taddr)
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, "
+      "%35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, "
+      "%52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+        "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+        "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+        "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+        "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
+        "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]),
+        "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]),
+        "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]),
+        "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -105,6 +117,20 @@ __device__ __forceinline__ void softmax_sync() {  // the four softmax warps
   asm volatile("bar.sync 1, 128;" ::: "memory");
 }
 
+// Two fp32 operations in one instruction, each rounded to nearest.
+__device__ __forceinline__ void fma2(float& x0, float& x1, float a, float b) {  // x a + b
+  asm("{\n\t.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\tmov.b64 z, {%3, %3};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(x0), "+f"(x1) : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void add2(float& x0, float& x1, float y0, float y1) {
+  asm("{\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(x0), "+f"(x1) : "f"(y0), "f"(y1));
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;
@@ -124,6 +150,14 @@ __device__ __forceinline__ float unpack(uint32_t w, int hi) {
 template <typename T>
 __device__ __forceinline__ constexpr uint32_t exp_mask() {
   return dtype_of<T>::value == 2 ? 0x7f80u : 0x7c00u;
+}
+
+// Scores of 64 keys, those that are not visible made -inf.
+__device__ __forceinline__ void mask_scores(uint32_t (&s)[64], uint32_t lo, uint32_t hi) {
+#pragma unroll
+  for (int j = 0; j < 64; ++j) {
+    s[j] = ((j < 32 ? lo : hi) >> (j & 31)) & 1u ? s[j] : 0xff800000u;
+  }
 }
 
 // Steps of 128 keys that block `blk` of the list needs, as a 4-bit set.
@@ -309,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
           for (int k = 0; k < kTile / 16; ++k) {
             // V (keys x D) is MN-major: 64-column slabs 16 KiB apart, 8-key groups 1 KiB
-            umma_f16_ts(tmem + 128, tmem + k * 8,
+            umma_f16_ts(tmem + 128, tmem + 64 + k * 8,
                         umma_smem_desc(vb + k * 2048, kTile * 128, 1024, 2), idesc_o,
                         (k != 0 || !fresh) ? 1u : 0u);
           }
@@ -368,26 +402,52 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
       }
       if (warp_live) {
-        float top = -INFINITY;
+        // The scores of keys 64..127 stay in registers from the maximum to the exponentials;
+        // those of keys 0..63 are read twice.  P goes over the second half's scores: keys
+        // 0..63 to columns 64..95, keys 64..127 to columns 96..127.
+        uint32_t s[64];
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          uint32_t s[32];
-          tmem_ld_32x32b_x32(tS + 32 * b, s);
+        for (int h = 0; h < 2; ++h) {
+          tmem_ld_x64(tS + 64 * h, s);
           tmem_ld_wait();
-          if (whole) {
+          if (!whole) mask_scores(s, vis[2 * h], vis[2 * h + 1]);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(s[j]));
-          } else {
+          for (int j = 0; j < 64; j += 8) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              top = fmaxf(top, (vis[b] >> j) & 1u ? __uint_as_float(s[j]) : -INFINITY);
+            for (int c = 0; c < 4; ++c) {
+              tops[c] = fmaxf(tops[c], fmaxf(__uint_as_float(s[j + 2 * c]),
+                                             __uint_as_float(s[j + 2 * c + 1])));
             }
           }
         }
+        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         const float t = top == -INFINITY ? top : top * p.scale_log2;
-        const bool move = t > m + kSlack || (m == -INFINITY && t > m);
+        const bool move = t > m + kSlack;  // (also from m = -inf)
         const float f = move ? exp2_approx(m - t) : 1.f;
         if (move) m = t;
+        const float base = m == -INFINITY ? 0.f : -m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 1; h >= 0; --h) {
+          if (h == 0) {
+            tmem_ld_x64(tS, s);
+            tmem_ld_wait();
+            if (!whole) mask_scores(s, vis[0], vis[1]);
+          }
+          uint32_t packed[32];
+#pragma unroll
+          for (int j = 0; j < 64; j += 2) {
+            float x0 = __uint_as_float(s[j]), x1 = __uint_as_float(s[j + 1]);
+            fma2(x0, x1, p.scale_log2, base);
+            x0 = exp2_approx(x0);
+            x1 = exp2_approx(x1);
+            add2(sum[j % 4], sum[j % 4 + 1], x0, x1);
+            packed[j / 2] = pack2<T>(x0, x1);
+          }
+          tmem_st_x32(tS + 64 + 32 * h, packed);
+        }
+        l = __fmaf_rn(l, f, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
         if (!fresh && __any_sync(0xffffffffu, move)) {
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
@@ -399,33 +459,6 @@ __global__ void __launch_bounds__(kThreads, 2)
             tmem_st_x32(tO + c, o);
           }
         }
-        const float base = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          uint32_t s[32];
-          tmem_ld_32x32b_x32(tS + 32 * b, s);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float x = exp2_approx(__fmaf_rn(__uint_as_float(s[j]), p.scale_log2, -base));
-            s[j] = __float_as_uint(x);
-          }
-          if (!whole) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) s[j] = (vis[b] >> j) & 1u ? s[j] : 0u;
-          }
-          uint32_t packed[16];
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float x0 = __uint_as_float(s[j]), x1 = __uint_as_float(s[j + 1]);
-            sum[j % 4] = __fadd_rn(sum[j % 4], x0);
-            sum[j % 4 + 1] = __fadd_rn(sum[j % 4 + 1], x1);
-            packed[j / 2] = pack2<T>(x0, x1);
-          }
-          tmem_st_x16(tS + 16 * b, packed);
-        }
-        l = __fmaf_rn(l, f, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
         tmem_st_wait();
       }
       if (!whole) {
@@ -480,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 2)
               if (((sh.bad[k >> 5] >> (k & 31)) & 1u) == 0) continue;
               __syncwarp();
               uint32_t pw;
-              tmem_ld_x1(tS + (k >> 1), pw);
+              tmem_ld_x1(tS + 64 + (k >> 1), pw);
               tmem_ld_wait();
               const float pk = unpack<T>(pw, k & 1);
               const uint32_t word = k < 32 ? vis[0] : k < 64 ? vis[1] : k < 96 ? vis[2] : vis[3];
