@@ -29,12 +29,14 @@ template <typename T, int DC>  // head dim 32 * DC
 __global__ void __launch_bounds__(kSimtThreads) paged_simt_kernel(const Params p) {
   constexpr int D = 32 * DC;
   constexpr int VEC = 16 / sizeof(T);
-  __shared__ SchedSmem<kSimtThreads> s_sched;
+  __shared__ SchedSmem<kSimtThreads, 1> s_sched;
   __shared__ float s_q[kSimtTile][D];
   grid_wait();
   grid_launch_dependents();
-  Work w;
-  if (!find_work<kSimtThreads>(p, blockIdx.x, s_sched, w, blockIdx.x == 0)) return;
+  find_work<kSimtThreads, 1>(p, blockIdx.x, s_sched, blockIdx.x == 0);
+  __syncthreads();
+  if (!s_sched.hit[0]) return;
+  const Work w = s_sched.found[0];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int subs = p.groups / p.Hkv;  // groups of a KV head
   const int head0 = w.kvh * p.G + (w.group % subs) * p.group_heads;
@@ -44,8 +46,8 @@ __global__ void __launch_bounds__(kSimtThreads) paged_simt_kernel(const Params p
   const int rows = n_tok * heads;
   const int pos0 = w.x.seq - w.x.n_tok + tok0;
   const BlockList list = block_list(p, pos0, pos0 + n_tok - 1);
-  const int i0 = static_cast<int>(static_cast<int64_t>(list.n) * w.piece / w.pieces);
-  const int i1 = static_cast<int>(static_cast<int64_t>(list.n) * (w.piece + 1) / w.pieces);
+  const int i0 = piece_start(list.n, w.piece, w.pieces);
+  const int i1 = piece_start(list.n, w.piece + 1, w.pieces);
   if (w.pieces > 1 && i0 == i1) return;
 
   for (int i = tid; i < rows * D; i += kSimtThreads) {
@@ -95,9 +97,10 @@ __global__ void __launch_bounds__(kSimtThreads) paged_simt_kernel(const Params p
       if (any == 0) continue;
       // this lane's key; a page outside the cache reads as zeros
       int64_t pg = -1;
-      if ((any >> lane) & 1u) pg = p.table[w.r * p.table_stride + key / p.page];
+      const int col = p.by_page(key);
+      if ((any >> lane) & 1u) pg = p.table[w.r * p.table_stride + col];
       const bool there = pg >= 0 && pg < p.n_pages;
-      const int64_t off = there ? key % p.page : 0;
+      const int64_t off = there ? key - col * p.page : 0;
       const T* krow = kbase + (there ? pg : 0) * p.ks[0] + off * p.ks[2];
       int64_t voff = (there ? pg : 0) * p.vs[0] + off * p.vs[2];
       float s[kSimtRows] = {};
@@ -224,12 +227,11 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     if (tok < x.tok || tok >= x.tok + x.n_tok) continue;
     const int4 info = p.info[r];
     if (info.x <= 1) continue;
-    const int64_t base = (static_cast<int64_t>(info.w) << 32) | static_cast<unsigned>(info.z);
-    const int in = tok - x.tok, tile = in / p.tile_tok;
+    const int in = tok - x.tok, tile = p.by_tile(in);
     const int pos0 = x.seq - x.n_tok + tile * p.tile_tok;
     const int n_tok = min(p.tile_tok, x.n_tok - tile * p.tile_tok);
     const BlockList list = block_list(p, pos0, pos0 + n_tok - 1);
-    const int64_t at = part_slot(p, base, info.y, in, head, 0);
+    const int64_t at = part_slot(p, info.z, info.y, in, head, 0);
     float m = -INFINITY, l = 0.f, o[DC];
 #pragma unroll
     for (int c = 0; c < DC; ++c) o[c] = 0.f;
@@ -368,20 +370,27 @@ int launch_paged_sdpa(const PagedSdpaArgs& a, cudaStream_t stream) {
   p.max_seq = std::min<int64_t>(a.width * a.page, INT32_MAX - kBlockKeys);
   p.group_heads = std::min(p.G, rows);
   p.tile_tok = rows / p.group_heads;
-  p.groups = p.Hkv * ((p.G + rows - 1) / rows);
+  const int subs = (p.G + rows - 1) / rows;
+  p.groups = p.Hkv * subs;
+  p.by_tile = divider(p.tile_tok);
+  p.by_page = divider(a.page);
+  p.by_head = divider(p.group_heads);
+  p.by_group = divider(subs);
   p.target = (tc ? 2 : 8) * device_sm_count();
   p.fine_rows = 16;
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   p.any_split = reinterpret_cast<int*>(ws);
   p.info = reinterpret_cast<int4*>(ws + 16);
   const int64_t left = a.workspace_bytes - info_bytes(a.R);
-  p.slots = left > 256 ? (left - 256) / (4 * a.D + 8) : 0;
+  p.slots = left <= 256 ? 0u : static_cast<unsigned>(
+      std::min<int64_t>((left - 256) / (4 * a.D + 8), kMuch - 1));
   p.part_o = reinterpret_cast<float*>(ws + info_bytes(a.R));
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + p.slots * a.D);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<int64_t>(p.slots) * a.D);
 
   // tiles of all requests: at most one ragged tile each
   const int64_t tiles = a.T / p.tile_tok + std::min(a.R, a.T);
-  const int64_t items = tiles * p.groups + 4LL * p.target + 1;
+  // (the spans are rounded in fp32: a little above 4 target pieces)
+  const int64_t items = tiles * p.groups + 4LL * p.target + 64;
   if (items > INT32_MAX) return set_error(BI_ERR_UNSUPPORTED, "too many query tiles");
   const int st = tc ? launch_paged_tc(a, p, items, stream)
                     : dispatch(p, a.dtype, a.D, items, false, stream);

@@ -57,6 +57,21 @@ __device__ __forceinline__ float row_value(float o, float scale) {
   return scale == 0.f ? 0.f : __fmaf_rn(o, scale, 0.f);
 }
 
+// Division of numbers below 2^31 by a fixed d in [1, 2^31): n mul >> shift with
+// mul = ceil(2^(31 + l) / d), l = ceil(log2 d) (exact: mul d - 2^(31 + l) < d <= 2^l).
+struct Divider {
+  unsigned d, mul, shift;
+  __device__ __forceinline__ int operator()(int n) const {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<unsigned>(n)) * mul) >> shift);
+  }
+};
+inline Divider divider(int64_t d) {
+  unsigned l = 0;
+  while ((1ll << l) < d) ++l;
+  const uint64_t top = 1ull << (31 + l);
+  return {static_cast<unsigned>(d), static_cast<unsigned>((top + d - 1) / d), 31 + l};
+}
+
 // What every kernel of the call knows.
 struct Params {
   const void* q;
@@ -79,18 +94,26 @@ struct Params {
   int64_t max_seq;         // tokens a row of the block table holds
   int tile_tok;            // tokens of a tile
   int groups, group_heads; // a KV head's query heads as groups (tiles cover one group)
+  Divider by_tile, by_page, by_head, by_group;  // tile_tok, page, group_heads, groups / Hkv
   int target;              // work items to aim for when a request's keys are split
   int fine_rows;           // tiles of at most so many rows are cheap to split
   // partial results of split requests
-  int4* info;              // per request {pieces, blocks a row has, base low, base high}
+  int4* info;              // per request {pieces, blocks a row has, first slot, -}
   int* any_split;
   float2* part_ml;         // (slot,) (m, l)
   float* part_o;           // (slot, D)
-  int64_t slots;
+  unsigned slots;
 };
 
 __device__ __forceinline__ int clampi(int64_t v, int64_t lo, int64_t hi) {
   return static_cast<int>(v < lo ? lo : (v > hi ? hi : v));
+}
+
+// Piece `piece` of `pieces` of a list of n blocks: [first, first of the next piece).
+__device__ __forceinline__ int piece_start(int n, int piece, int pieces) {
+  if (pieces == 1) return piece == 0 ? 0 : n;
+  const unsigned each = static_cast<unsigned>(n) / static_cast<unsigned>(pieces);
+  return piece * static_cast<int>(each) + min(piece, n - static_cast<int>(each) * pieces);
 }
 
 // The key blocks that the queries at positions [pmin, pmax] need: block i of the list is
@@ -127,11 +150,11 @@ __device__ __forceinline__ Request request(const Params& p, int r) {
   return x;
 }
 __device__ __forceinline__ int tiles_of(const Params& p, const Request& x) {
-  return (x.n_tok + p.tile_tok - 1) / p.tile_tok;
+  return p.by_tile(x.n_tok + p.tile_tok - 1);
 }
 // Most key blocks that any of its tiles lists.
 __device__ __forceinline__ int blocks_of(const Params& p, const Request& x) {
-  const int all = x.seq / kBlockKeys + (x.seq % kBlockKeys != 0);
+  const int all = (x.seq + kBlockKeys - 1) / kBlockKeys;
   if (p.window == INT32_MAX) return all;
   const int64_t keys = static_cast<int64_t>(p.window) + min(p.tile_tok, x.n_tok);
   const int64_t most = p.first / kBlockKeys + keys / kBlockKeys + 3;
@@ -141,134 +164,198 @@ __device__ __forceinline__ int blocks_of(const Params& p, const Request& x) {
 struct Work {
   int r, tile, group, kvh, piece, pieces;
   int blocks;        // most blocks a row of the request has
-  int64_t base;      // first slot of the request's partial results (pieces > 1)
+  int base;          // first slot of the request's partial results (pieces > 1)
   Request x;
 };
 
-template <int NT>
+// The work of a block: ITEMS consecutive items of the call.
+template <int NT, int ITEMS>
 struct SchedSmem {
-  int64_t a[NT / 32], b[NT / 32];
-  Work found;
-  int hit;
+  float f[NT / 32];
+  unsigned a[NT / 32], b[NT / 32];
+  Work found[ITEMS];
+  int hit[ITEMS];
 };
 
-template <int NT>
-__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* s) {
+constexpr unsigned kMuch = 1u << 30;  // sums of slots stop here (the workspace holds fewer)
+__device__ __forceinline__ unsigned add_sat(unsigned a, unsigned b) { return min(a + b, kMuch); }
+
+__device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int d = 16; d > 0; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-  __syncthreads();
-  int64_t t = 0;
-#pragma unroll
-  for (int w = 0; w < NT / 32; ++w) t += s[w];
-  __syncthreads();
-  return t;
+  return v;
 }
-
-// Exclusive scan over the block; `total` receives the sum.
-template <int NT>
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* s, int64_t& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t inc = v;
+// Inclusive scans of item counts and (saturating) slot counts over a warp.
+__device__ __forceinline__ void warp_scan(unsigned& a, unsigned& b, int lane) {
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
-    const int64_t o = __shfl_up_sync(0xffffffffu, inc, d);
-    if (lane >= d) inc += o;
+    const unsigned x = __shfl_up_sync(0xffffffffu, a, d), y = __shfl_up_sync(0xffffffffu, b, d);
+    if (lane >= d) {
+      a += x;
+      b = add_sat(b, y);
+    }
   }
-  if (lane == 31) s[warp] = inc;
-  __syncthreads();
-  int64_t before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < NT / 32; ++w) {
-    if (w < warp) before += s[w];
-    total += s[w];
-  }
-  __syncthreads();
-  return before + inc - v;
 }
 
-// Work item `item` of the call, found by the whole block (NT threads); false: there is none.
-// Items go request by request, in a request group of heads by group, tile by tile from the
-// last (in causal attention the longest) to the first, piece by piece of the tile's keys.
+// Into how many pieces the keys of a request's tiles are split, and the slots that its partial
+// results then take.
 //
-// A request's keys are split into pieces only where that shortens the call: a tile whose
-// blocks are at most the average load of a block slot is computed by one block, which then
-// keeps the fold in registers.  Requests whose tiles have few rows (decode), whose partial
-// results are small beside the keys they stand for, are split four times finer, so that
-// ragged lengths spread evenly.  The choice changes no bit of the results.
-template <int NT>
-__device__ __forceinline__ bool find_work(const Params& p, int64_t item, SchedSmem<NT>& s,
-                                          Work& out, bool publish) {
-  const int tid = threadIdx.x;
-  if (tid == 0) s.hit = 0;
-  int64_t load = 0;
-  for (int r = tid; r < p.R; r += NT) {
-    const Request x = request(p, r);
-    load += static_cast<int64_t>(tiles_of(p, x)) * blocks_of(p, x);
+// A request's keys are split only where that shortens the call: a tile whose blocks are at
+// most the average load (`span`) is computed in one go, which then keeps the fold in
+// registers.  Requests whose tiles have few rows (decode), whose partial results are small
+// beside the keys they stand for, are split four times finer (`fine`), so that ragged lengths
+// spread evenly.  The choice changes no bit of the results.
+struct Spans {
+  unsigned span, fine;
+};
+__device__ __forceinline__ Spans spans_of(const Params& p, float load) {
+  load *= static_cast<float>(p.groups);
+  const float t = static_cast<float>(p.target);
+  return {static_cast<unsigned>(fmaxf(1.f, ceilf(load / t))),
+          static_cast<unsigned>(fmaxf(1.f, ceilf(load / (4.f * t))))};
+}
+__device__ __forceinline__ float load_of(const Params& p, const Request& x) {
+  return static_cast<float>(tiles_of(p, x)) * static_cast<float>(blocks_of(p, x));
+}
+__device__ __forceinline__ unsigned pieces_of(const Params& p, const Request& x, const Spans& s,
+                                              int tiles, int blocks, unsigned& slots) {
+  const unsigned most = min(x.n_tok, p.tile_tok) * p.group_heads <= p.fine_rows ? s.fine : s.span;
+  const unsigned pieces = tiles == 0 ? 0 : max(1u, (blocks + most - 1) / most);
+  const float want = static_cast<float>(x.n_tok) * static_cast<float>(p.H) *
+                     static_cast<float>(blocks);
+  slots = pieces <= 1 ? 0u : want >= static_cast<float>(kMuch) ? kMuch
+                                 : static_cast<unsigned>(x.n_tok) * p.H * blocks;
+  return pieces;
+}
+
+// One request's share of the search: its items are [at, at + items).
+template <int NT, int ITEMS>
+__device__ __forceinline__ void take_items(const Params& p, int item, SchedSmem<NT, ITEMS>& s,
+                                           int r, const Request& x, int tiles, int blocks,
+                                           unsigned pieces, unsigned base, unsigned at,
+                                           unsigned items) {
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const unsigned i = static_cast<unsigned>(item + k);
+    if (i < at || i >= at + items) continue;
+    const unsigned in = i - at, per_group = tiles * pieces;
+    Work w;
+    w.r = r;
+    w.pieces = pieces;
+    w.blocks = blocks;
+    w.base = base;
+    w.x = x;
+    w.group = in / per_group;
+    const unsigned rest = in - w.group * per_group;
+    w.tile = tiles - 1 - static_cast<int>(rest / pieces);
+    w.piece = rest % pieces;
+    w.kvh = p.by_group(w.group);
+    s.found[k] = w;
+    s.hit[k] = 1;
   }
-  load = block_sum<NT>(load, s.a) * p.groups;
-  const int64_t span = max(static_cast<int64_t>(1), (load + p.target - 1) / p.target);
-  const int64_t fine = max(static_cast<int64_t>(1), (load + 4 * p.target - 1) / (4 * p.target));
-  int64_t items0 = 0, slots0 = 0;
-  int split = 0;
-  for (int r0 = 0; r0 < p.R; r0 += NT) {
-    const int r = r0 + tid;
-    Request x{0, 0, 0};
-    int64_t items = 0, slots = 0;
-    int pieces = 0, blocks = 0, tiles = 0;
-    if (r < p.R) {
-      x = request(p, r);
-      tiles = tiles_of(p, x);
-      blocks = blocks_of(p, x);
-      const int64_t rows = static_cast<int64_t>(min(x.n_tok, p.tile_tok)) * p.group_heads;
-      const int64_t most = rows <= p.fine_rows ? fine : span;
-      pieces = tiles > 0 ? static_cast<int>(max(static_cast<int64_t>(1),
-                                                (blocks + most - 1) / most)) : 0;
-      if (pieces > 1) slots = static_cast<int64_t>(x.n_tok) * p.H * blocks;
+}
+
+// Finds items item .. item + ITEMS - 1 of the call, with all threads of the block (NT); the
+// answer is in `s` after the block's next barrier.  Items go request by request, in a request
+// group of heads by group, tile by tile from the last (in causal attention the longest) to the
+// first, piece by piece of a tile's keys.  Up to 64 requests one warp does it in registers;
+// beyond, the block scans them 32 a warp at a time.  The block that `publish`es leaves the
+// split of every request for the join.
+template <int NT, int ITEMS>
+__device__ __forceinline__ void find_work(const Params& p, int item, SchedSmem<NT, ITEMS>& s,
+                                          bool publish) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (p.R <= 64) {
+    if (warp != 0) return;
+    if (lane < ITEMS) s.hit[lane] = 0;
+    __syncwarp();
+    Request x[2];
+    float load = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = lane + 32 * h;
+      x[h] = r < p.R ? request(p, r) : Request{0, 0, 0};
+      load += load_of(p, x[h]);
     }
-    int64_t total;
-    const int64_t base = slots0 + block_scan<NT>(slots, s.b, total);
-    slots0 += total;
-    if (pieces > 1 && base + slots > p.slots) pieces = 1;  // no room for its partial results
-    items = static_cast<int64_t>(tiles) * pieces * p.groups;
-    const int64_t at = items0 + block_scan<NT>(items, s.a, total);
-    items0 += total;
-    if (r < p.R && publish) {
-      p.info[r] = make_int4(pieces, blocks, static_cast<int>(base & 0xffffffff),
-                            static_cast<int>(base >> 32));
+    const Spans sp = spans_of(p, warp_sum(load));
+    unsigned items0 = 0, slots0 = 0, split = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = lane + 32 * h, tiles = tiles_of(p, x[h]), blocks = blocks_of(p, x[h]);
+      unsigned slots;
+      unsigned pieces = pieces_of(p, x[h], sp, tiles, blocks, slots);
+      unsigned none = 0, ends = slots;
+      warp_scan(none, ends, lane);
+      const unsigned base = add_sat(slots0, ends) - slots;  // (exact below kMuch)
+      if (pieces > 1 && add_sat(slots0, ends) > p.slots) pieces = 1;
+      const unsigned items = tiles * pieces * p.groups;
+      unsigned at = items;
+      warp_scan(at, none, lane);
+      slots0 = add_sat(slots0, __shfl_sync(0xffffffffu, ends, 31));
+      take_items(p, item, s, r, x[h], tiles, blocks, pieces, base, items0 + at - items, items);
+      items0 += __shfl_sync(0xffffffffu, at, 31);
+      if (publish && r < p.R) p.info[r] = make_int4(pieces, blocks, base, 0);
       split |= pieces > 1;
     }
-    if (item >= at && item < at + items) {
-      const int64_t in = item - at;
-      Work w;
-      w.r = r;
-      w.pieces = pieces;
-      w.blocks = blocks;
-      w.base = base;
-      w.x = x;
-      const int per_group = tiles * pieces;
-      w.group = static_cast<int>(in / per_group);
-      const int rest = static_cast<int>(in - static_cast<int64_t>(w.group) * per_group);
-      w.tile = tiles - 1 - rest / pieces;
-      w.piece = rest % pieces;
-      w.kvh = w.group / (p.groups / p.Hkv);
-      s.found = w;
-      s.hit = 1;
+    if (publish) {
+      split = __any_sync(0xffffffffu, split);
+      if (lane == 0) *p.any_split = split;
     }
-    if (!publish && items0 > item) break;  // (uniform)
+    return;
+  }
+  if (tid < ITEMS) s.hit[tid] = 0;
+  float load = 0.f;
+  for (int r = tid; r < p.R; r += NT) load += load_of(p, request(p, r));
+  load = warp_sum(load);
+  if (lane == 0) s.f[warp] = load;
+  __syncthreads();
+  load = 0.f;
+#pragma unroll
+  for (int w = 0; w < NT / 32; ++w) load += s.f[w];
+  const Spans sp = spans_of(p, load);
+  unsigned items0 = 0, slots0 = 0, split = 0;
+  for (int r0 = 0; r0 < p.R; r0 += NT) {
+    const int r = r0 + tid;
+    const Request x = r < p.R ? request(p, r) : Request{0, 0, 0};
+    const int tiles = tiles_of(p, x), blocks = blocks_of(p, x);
+    unsigned slots, none = 0;
+    unsigned pieces = pieces_of(p, x, sp, tiles, blocks, slots);
+    unsigned ends = slots;
+    warp_scan(none, ends, lane);
+    if (lane == 31) s.b[warp] = ends;
+    __syncthreads();
+    unsigned total = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) {
+      if (w == warp) ends = add_sat(ends, add_sat(slots0, total));
+      total = add_sat(total, s.b[w]);
+    }
+    slots0 = add_sat(slots0, total);
+    if (pieces > 1 && ends > p.slots) pieces = 1;  // no room for its partial results
+    const unsigned items = tiles * pieces * p.groups;
+    unsigned at = items;
+    warp_scan(at, none, lane);
+    if (lane == 31) s.a[warp] = at;
+    __syncthreads();
+    at += items0 - items;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) {
+      if (w < warp) at += s.a[w];
+      items0 += s.a[w];
+    }
+    take_items(p, item, s, r, x, tiles, blocks, pieces, ends - slots, at, items);
+    if (publish && r < p.R) p.info[r] = make_int4(pieces, blocks, ends - slots, 0);
+    split |= pieces > 1;
+    if (!publish && items0 >= static_cast<unsigned>(item + ITEMS)) break;  // (uniform)
   }
   if (publish) {
     split = __syncthreads_or(split);
     if (tid == 0) *p.any_split = split;
   }
-  __syncthreads();
-  out = s.found;
-  return s.hit != 0;
 }
 
 // Slot of the partial result of (row, block i of its tile's list).
-__device__ __forceinline__ int64_t part_slot(const Params& p, int64_t base, int blocks,
+__device__ __forceinline__ int64_t part_slot(const Params& p, int base, int blocks,
                                              int tok_in_request, int head, int i) {
   return base + (static_cast<int64_t>(tok_in_request) * p.H + head) * blocks + i;
 }

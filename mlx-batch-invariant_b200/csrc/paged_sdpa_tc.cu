@@ -1,15 +1,20 @@
 // Attention of new tokens over a KV cache in pages on the 5th-generation tensor cores:
 // fp16 / bf16, head dim 64 or 128, page sizes that divide or are multiples of 128.
 //
-// A block (two per SM) takes one tile of 128 rows -- 128 / G tokens x the G query heads of a
-// KV head -- and walks the tile's keys 128 at a time:
-//   warp 4      TMA producer: the tile's q rows once, then K and V of each 128 keys, one box
-//               per page (the lanes fetch the pages' numbers one tile ahead);
-//   warp 5      tcgen05.mma: S = Q K^T (128 x 128, fp32 in TMEM) and O += P V with P read
-//               from TMEM;
-//   warps 0..3  one row per thread: maximum, exponentials, sum; P, rounded to the 16-bit
-//               type, goes back to TMEM over the scores it came from.
-// While one block's softmax runs the other block's products keep the tensor pipe busy.
+// A block (one per SM) works on two items at a time, each a tile of 128 rows -- 128 / G tokens
+// x the G query heads of a KV head -- whose keys it walks 128 at a time.  Neighbouring tiles
+// of a long chunk share the K and V tiles; otherwise (decode) the two items have their own:
+//   warp 8      TMA producer: the tiles' q rows once, then K and V tiles, one box per page
+//               (the lanes fetch the pages' numbers ahead), through one ring;
+//   warp 9      tcgen05.mma: S = Q K^T (128 x 128, fp32 in TMEM) and O += P V with P read
+//               from TMEM, the two items' products in turn;
+//   warps 0..3 and 4..7  softmax of the first and of the second item, one row per thread:
+//               maximum, exponentials, sum; P, rounded to the 16-bit type, goes back to TMEM
+//               over the scores it came from.
+// One thread issues both items' products in turn, so while one item's products run the other's
+// softmax does: two blocks per SM with an item each fell into step, both in their softmax at
+// one time and both waiting for the tensor pipe at another (5000 clocks for two tiles of 128
+// keys where the products take 2048).
 //
 // The running maximum of a 512-key block only moves when a tile's exceeds it by more than
 // 2^8: until then the weights are up to 256 times too large, which the 16-bit type and the
@@ -26,12 +31,13 @@ namespace bi {
 namespace psdpa {
 namespace tcp {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 384;
 constexpr int kTile = 128;            // rows of a tile and keys of a step
-constexpr int kRegsSoftmax = 208;     // 128 x (208 + 48) = 256 x 128, the launch's registers
-constexpr int kRegsOther = 48;
-constexpr int kTmemCols = 256;        // S at 0 (P over its second half), O at 128
+constexpr int kRegsSoftmax = 216;     // 2 x 216 + 72 = 3 x 168, the launch's registers
+constexpr int kRegsOther = 72;
+constexpr int kTmemCols = 512;        // per item: S (P over its second half) and O, 128 each
 constexpr float kSlack = 8.f;         // log 2 of how far weights may exceed 1
+constexpr int kMaxStages = 12;
 
 enum : unsigned { kSiteProducer = 1, kSiteMma = 2, kSiteSoftmax = 3, kSiteDrain = 4 };
 
@@ -41,17 +47,8 @@ template <int D>
 struct Cfg {
   static constexpr int kHalves = D / 64;
   static constexpr int kTileBytes = kTile * D * 2;
-  static constexpr int kStages = D == 128 ? 2 : 4;  // K and V tiles alternate
-  static constexpr int kSmem = 1024 + (1 + kStages) * kTileBytes;
-};
-
-struct Shared {
-  SchedSmem<kThreads> sched;
-  uint64_t q_full, full[4], empty[4], s_full, p_ready, o_full, mma_done;
-  uint32_t tmem;
-  int abort_flag;
-  int keep_o;         // the softmax warps put values into O: accumulate on them
-  unsigned bad[4];    // keys of the tile with a non-finite value that some row sees
+  static constexpr int kStages = D == 128 ? 5 : 12;  // K and V tiles
+  static constexpr int kSmem = 1024 + (2 + kStages) * kTileBytes;
 };
 
 __device__ __forceinline__ void tmem_ld_x1(uint32_t taddr, uint32_t& r) {
@@ -97,12 +94,12 @@ __device__ __forceinline__ void tmem_st_wait() {
 }
 // D(tmem) (+)= A(tmem) x B(smem desc)
 __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
-                                            uint32_t idesc, uint32_t accumulate) {
+                                            uint32_t idesc, bool accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
       : "memory");
 }
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar,
@@ -113,8 +110,42 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
-__device__ __forceinline__ void softmax_sync() {  // the four softmax warps
-  asm volatile("bar.sync 1, 128;" ::: "memory");
+// The four softmax warps of an item, or (both) those of the two items.
+// A whole warp's wait, bounded like mbar_wait; a loop of few instructions (the kernel's code
+// has to stay within the instruction cache: at 142 KB every step of it was fetched anew, and
+// the kernel ran no faster than its code came in).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity,
+                                          const volatile int* abort_flag) {
+  const uint32_t addr = smem_u32(bar);
+  bool ok = true;
+  long long start = 0;
+#pragma unroll 1
+  for (uint32_t it = 0; !mbar_try_wait(addr, parity); ++it) {
+    if ((it & 255u) == 255u) {
+      const long long now = clock64();
+      if (start == 0) start = now;
+      if (*abort_flag || now - start > kWaitBudgetCycles) {
+        ok = false;
+        break;
+      }
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+// One lane of the converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(yes));
+  return yes != 0;
+}
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ void softmax_sync(int item, bool both) {
+  if (both) {
+    asm volatile("bar.sync 3, 256;" ::: "memory");
+  } else {
+    asm volatile("bar.sync %0, 128;" ::"r"(1 + item) : "memory");
+  }
 }
 
 // Two fp32 operations in one instruction, each rounded to nearest.
@@ -152,46 +183,113 @@ __device__ __forceinline__ constexpr uint32_t exp_mask() {
   return dtype_of<T>::value == 2 ? 0x7f80u : 0x7c00u;
 }
 
-// Scores of 64 keys, those that are not visible made -inf.
-__device__ __forceinline__ void mask_scores(uint32_t (&s)[64], uint32_t lo, uint32_t hi) {
-#pragma unroll
-  for (int j = 0; j < 64; ++j) {
-    s[j] = ((j < 32 ? lo : hi) >> (j & 31)) & 1u ? s[j] : 0xff800000u;
-  }
-}
+// What one of a block's two items is.
+struct Item {
+  int pieces;             // 0: it is not there
+  int r, kvh, tok, base, blocks;  // request, KV head, first row, Work's base and blocks
+  int n_tok, rows, tok0;  // its tile (tok0 in the request)
+  int pos0, pmax;         // positions of its first and last token
+  // the keys it walks: blocks [i0, i1) of `list`.  Items that share K and V walk the keys that
+  // either needs; what a row does not see changes nothing.
+  BlockList list;
+  int list_pos0, list_pmax;
+  int i0, i1;
+  int steps;              // of 128 keys
+};
 
 // Steps of 128 keys that block `blk` of the list needs, as a 4-bit set.
-__device__ __forceinline__ unsigned steps_of(const Params& p, const BlockList& list, int pmax,
-                                             int blk) {
+__device__ __forceinline__ unsigned steps_of(const Params& p, const Item& it, int blk) {
   unsigned set = 0;
 #pragma unroll
   for (int s = 0; s < kBlockKeys / kTile; ++s) {
     const int t0 = blk * kBlockKeys + s * kTile;
-    if (t0 <= pmax && (t0 + kTile > list.lo_key || t0 < p.first)) set |= 1u << s;
+    if (t0 <= it.list_pmax && (t0 + kTile > it.list.lo_key || t0 < p.first)) set |= 1u << s;
   }
   return set;
 }
 
-// The next step behind (i, s) of the blocks [.., i1): its first key, or -1.
+// Describes item k of the block; a whole warp.
+__device__ __forceinline__ void make_item(const Params& p, const SchedSmem<kThreads, 2>& s, int k,
+                                          bool shared, Item& out) {
+  const int lane = threadIdx.x & 31;
+  Item it;
+  it.pieces = 0;
+  it.r = it.kvh = it.tok = it.base = it.blocks = 0;
+  it.n_tok = it.rows = it.tok0 = it.pos0 = it.i0 = it.i1 = it.steps = 0;
+  it.pmax = it.list_pos0 = it.list_pmax = -1;
+  it.list = BlockList{0, 0, 0, 0};
+  if (s.hit[k]) {
+    const Work& w = s.found[k];
+    it.pieces = w.pieces;
+    it.r = w.r;
+    it.kvh = w.kvh;
+    it.base = w.base;
+    it.blocks = w.blocks;
+    it.tok0 = w.tile * p.tile_tok;
+    it.tok = w.x.tok + it.tok0;
+    it.n_tok = min(p.tile_tok, w.x.n_tok - it.tok0);
+    it.rows = it.n_tok * p.G;
+    const int first = w.x.seq - w.x.n_tok;
+    it.pos0 = first + it.tok0;
+    it.pmax = it.pos0 + it.n_tok - 1;
+    it.list_pos0 = it.pos0;
+    it.list_pmax = it.pmax;
+    if (shared) {  // item 1 is the tile before item 0's
+      it.list_pos0 = first + s.found[1].tile * p.tile_tok;
+      it.list_pmax = first + min((s.found[0].tile + 1) * p.tile_tok, w.x.n_tok) - 1;
+    }
+    it.list = block_list(p, it.list_pos0, it.list_pmax);
+    it.i0 = piece_start(it.list.n, w.piece, w.pieces);
+    it.i1 = piece_start(it.list.n, w.piece + 1, w.pieces);
+    unsigned n = 0;
+    for (int i = it.i0 + lane; i < it.i1; i += 32) n += __popc(steps_of(p, it, it.list.at(i)));
+    it.steps = static_cast<int>(__reduce_add_sync(0xffffffffu, n));
+  }
+  if (lane == 0) out = it;
+}
+
+// Walks an item's steps.
 struct StepIter {
-  int i, i1;
-  unsigned left;  // steps of block i still to come
+  int i;
+  unsigned left;  // steps of the block still to come
   int blk;
 };
-__device__ __forceinline__ int next_step(const Params& p, const BlockList& list, int pmax,
-                                         StepIter& it) {
+// The first key of the next step, or -1.
+__device__ __forceinline__ int next_step(const Params& p, const Item& item, StepIter& it) {
   while (it.left == 0) {
-    if (it.i >= it.i1) return -1;
-    it.blk = list.at(it.i++);
-    it.left = steps_of(p, list, pmax, it.blk);
+    if (it.i >= item.i1) return -1;
+    it.blk = item.list.at(it.i++);
+    it.left = steps_of(p, item, it.blk);
   }
   const int s = __ffs(it.left) - 1;
   it.left &= it.left - 1;
   return it.blk * kBlockKeys + s * kTile;
 }
 
+// The order of the K and V tiles in the ring, which the producer fills and the products empty:
+// shared, K(0) V(0) K(1) V(1) ...; else the items' K(0), then round by round V(j) and K(j + 1)
+// of item 0, then of item 1.  Place of V(j) of item k:
+__device__ __forceinline__ int v_place(bool shared, int l0, int l1, int k, int j) {
+  if (shared) return 2 * j + 1;
+  int n = (l0 > 0) + (l1 > 0) + min(j, l0) + min(j, max(l0 - 1, 0)) + min(j, l1) +
+          min(j, max(l1 - 1, 0));
+  if (k == 1) n += (j < l0) + (j + 1 < l0);
+  return n;
+}
+
+struct Shared {
+  SchedSmem<kThreads, 2> sched;
+  uint64_t q_full[2], full[kMaxStages], empty[kMaxStages], s_full[2], p_ready[2], o_full[2],
+      mma_done;
+  uint32_t tmem;
+  int abort_flag;
+  Item item[2];
+  int keep_o[2];          // the softmax warps put values into O: accumulate on them
+  unsigned bad[2][2][4];  // keys of a step with a non-finite value that some row sees
+};
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 1)
     paged_tc_kernel(const __grid_constant__ CUtensorMap map_q,
                     const __grid_constant__ CUtensorMap map_q1,
                     const __grid_constant__ CUtensorMap map_k,
@@ -202,195 +300,272 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* s_q = smem;
-  uint8_t* s_ring = smem + C::kTileBytes;
+  uint8_t* s_ring = smem + 2 * C::kTileBytes;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* abort_flag = &sh.abort_flag;
 
+  if (warp == 8 && lane == 0) {
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_q1);
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
   grid_wait();
   grid_launch_dependents();
-  Work w;
-  if (!find_work<kThreads>(p, blockIdx.x, sh.sched, w, blockIdx.x == 0)) return;
-  const int tok0 = w.tile * p.tile_tok;  // in the request
-  const int n_tok = min(p.tile_tok, w.x.n_tok - tok0);
-  const int rows = n_tok * p.G;
-  const int pos0 = w.x.seq - w.x.n_tok + tok0;
-  const int pmax = pos0 + n_tok - 1;
-  const BlockList list = block_list(p, pos0, pmax);
-  const int i0 = static_cast<int>(static_cast<int64_t>(list.n) * w.piece / w.pieces);
-  const int i1 = static_cast<int>(static_cast<int64_t>(list.n) * (w.piece + 1) / w.pieces);
-  if (w.pieces > 1 && i0 == i1) return;
+  find_work<kThreads, 2>(p, 2 * blockIdx.x, sh.sched, blockIdx.x == 0);
+  __syncthreads();
+  if (!sh.sched.hit[0]) return;
+  // two tiles of one request and group, their keys not split: they share K and V
+  const bool shared = sh.sched.hit[1] && sh.sched.found[0].r == sh.sched.found[1].r &&
+                      sh.sched.found[0].group == sh.sched.found[1].group &&
+                      sh.sched.found[0].pieces == 1;
 
   if (tid == 0) {
-    mbar_init(&sh.q_full, 1);
+    for (int k = 0; k < 2; ++k) {
+      mbar_init(&sh.q_full[k], 1);
+      mbar_init(&sh.s_full[k], 1);
+      mbar_init(&sh.p_ready[k], 4);
+      mbar_init(&sh.o_full[k], 1);
+      sh.keep_o[k] = 0;
+    }
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&sh.full[s], 1);
-      mbar_init(&sh.empty[s], 1);
+      mbar_init(&sh.empty[s], shared ? 2 : 1);
     }
-    mbar_init(&sh.s_full, 1);
-    mbar_init(&sh.p_ready, 4);
-    mbar_init(&sh.o_full, 1);
     mbar_init(&sh.mma_done, 1);
     sh.abort_flag = 0;
-    sh.keep_o = 0;
     fence_barrier_init();
   }
-  if (warp == 5) {
+  if (warp == 9) {
     tmem_alloc(&sh.tmem, kTmemCols);
     tmem_relinquish();
   }
+  if (warp == 4 || warp == 7) make_item(p, sh.sched, warp == 7, shared, sh.item[warp == 7]);
   __syncwarp();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
 
-  if (warp >= 4) {
+  if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-    if (warp == 4) {
+    if (warp == 8) {
       // ---------------- TMA producer ----------------
-      if (lane == 0 && i0 < i1) {
+      const int side = lane >> 4, sub = lane & 15;  // 16 lanes per item
+      const Item item = sh.item[side];
+      if (sub == 0 && item.steps > 0) {
         // a decoding request's one token, or the tile's (and, behind the request's last,
         // other requests': rows that are computed and not stored)
-        const bool single = n_tok == 1;
-        mbar_arrive_expect_tx(&sh.q_full, static_cast<uint32_t>(
+        const bool single = item.n_tok == 1;
+        mbar_arrive_expect_tx(&sh.q_full[side], static_cast<uint32_t>(
             (single ? 1 : p.tile_tok) * p.G * D * 2));
         for (int h = 0; h < C::kHalves; ++h) {
-          tma_load_3d(s_q + h * (kTile * 128), single ? &map_q1 : &map_q, &sh.q_full, h * 64,
-                      w.kvh * p.G, w.x.tok + tok0);
+          tma_load_3d(s_q + side * C::kTileBytes + h * (kTile * 128), single ? &map_q1 : &map_q,
+                      &sh.q_full[side], h * 64, item.kvh * p.G, item.tok);
         }
       }
+      __syncwarp();
       const int box_rows = min(p.page, kTile);
       const int n_box = kTile / box_rows;
-      const int* entries = p.table + static_cast<int64_t>(w.r) * p.table_stride;
+      const int* entries = p.table + static_cast<int64_t>(item.r) * p.table_stride;
+      const int kvh = item.kvh;
       auto page_of = [&](int t0) {  // of this lane's box; n_pages (zero fill) where none is
-        if (t0 < 0 || lane >= n_box) return p.n_pages;
-        const int key = t0 + lane * box_rows;
-        if (key > pmax) return p.n_pages;
-        const int pg = entries[key / p.page];
+        if (t0 < 0 || sub >= n_box) return p.n_pages;
+        const int key = t0 + sub * box_rows;
+        if (key > item.list_pmax) return p.n_pages;
+        const int pg = entries[p.by_page(key)];
         return pg >= 0 && pg < p.n_pages ? pg : p.n_pages;
       };
-      StepIter it{i0, i1, 0, 0};
-      int t0 = next_step(p, list, pmax, it);
-      int pg = page_of(t0);
       int n = 0;
-      bool ok = true, any = false;
-      while (t0 >= 0 && ok) {
-        const int nt = next_step(p, list, pmax, it);
-        const int npg = page_of(nt);
-        const int row = (t0 + lane * box_rows) % p.page;
+      bool ok = true;
+      auto load = [&](const CUtensorMap* map, int k, int t0, int pg) {
+        const int stage = n % C::kStages;
+        ok = ok && warp_wait(&sh.empty[stage], ((n / C::kStages) & 1) ^ 1u, abort_flag);
+        ++n;
+        if (!ok) return;
+        if (lane == 0) mbar_arrive_expect_tx(&sh.full[stage], C::kTileBytes);
+        __syncwarp();
+        if (side == k && sub < n_box) {
+          uint8_t* dst = s_ring + stage * C::kTileBytes + sub * box_rows * 128;
+          const int key = t0 + sub * box_rows, row = key - p.by_page(key) * p.page;
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv, ++n) {
-          const int stage = n % C::kStages;
-          const uint32_t phase = (n / C::kStages) & 1;
-          ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[stage], phase ^ 1u, abort_flag));
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&sh.full[stage], C::kTileBytes);
-          __syncwarp();
-          if (lane < n_box) {
-            uint8_t* dst = s_ring + stage * C::kTileBytes + lane * box_rows * 128;
-#pragma unroll
-            for (int h = 0; h < C::kHalves; ++h) {
-              tma_load_4d(dst + h * (kTile * 128), kv == 0 ? &map_k : &map_v, &sh.full[stage],
-                          h * 64, row, w.kvh, pg);
-            }
+          for (int h = 0; h < C::kHalves; ++h) {
+            tma_load_4d(dst + h * (kTile * 128), map, &sh.full[stage], h * 64, row, kvh, pg);
           }
-          any = true;
         }
-        t0 = nt;
-        pg = npg;
+      };
+      const int l0 = sh.item[0].steps, l1 = shared ? 0 : sh.item[1].steps, rounds = max(l0, l1);
+      StepIter it{item.i0, 0, 0};
+      int t0 = next_step(p, item, it), t1 = t0 < 0 ? -1 : next_step(p, item, it);
+      int pg0 = page_of(t0), pg1 = page_of(t1);
+      if (l0 > 0) load(&map_k, 0, t0, pg0);
+      if (l1 > 0) load(&map_k, 1, t0, pg0);
+      for (int j = 0; j < rounds && ok; ++j) {
+        const int t2 = t1 < 0 ? -1 : next_step(p, item, it);
+        const int pg2 = page_of(t2);
+        if (j < l0) load(&map_v, 0, t0, pg0);
+        if (j + 1 < l0) load(&map_k, 0, t1, pg1);
+        if (j < l1) load(&map_v, 1, t0, pg0);
+        if (j + 1 < l1) load(&map_k, 1, t1, pg1);
+        t0 = t1;
+        t1 = t2;
+        pg0 = pg1;
+        pg1 = pg2;
       }
-      if (!ok && lane == 0) {
-        *abort_flag = 1;
-        record_error(&g_error_word_tc, (kSiteProducer << 8) | kErrReasonTimeout);
-      }
-      if (!ok && any) sleep_ns(200000);  // the copies in flight land
-    } else if (warp == 5) {
-      // ---------------- tcgen05.mma ----------------
-      if (lane == 0) {
-        constexpr uint32_t fmt = dtype_of<T>::value == 2 ? 1u : 0u;
-        constexpr uint32_t idesc_s = umma_idesc_f16(fmt, 0u, kTile, kTile);
-        constexpr uint32_t idesc_o = umma_idesc_f16(fmt, 1u, kTile, D);
-        StepIter it{i0, i1, 0, 0};
-        bool ok = true;
-        int n = 0, step = 0;
-        if (i0 < i1) ok = mbar_wait(&sh.q_full, 0, abort_flag);
-        bool fresh = true;  // the next product starts a key block
-        for (int t0 = next_step(p, list, pmax, it); ok && t0 >= 0; ++step) {
-          int stage = n % C::kStages;
-          ok = mbar_wait(&sh.full[stage], (n / C::kStages) & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t qb = smem_u32(s_q), kb = smem_u32(s_ring + stage * C::kTileBytes);
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = (k / 4) * (kTile * 128) + (k % 4) * 32;
-            umma_f16(tmem, umma_smem_desc(qb + off, 16, 1024, 2),
-                     umma_smem_desc(kb + off, 16, 1024, 2), idesc_s, k != 0 ? 1u : 0u);
-          }
-          umma_commit(&sh.empty[stage]);
-          umma_commit(&sh.s_full);
-          ++n;
-          stage = n % C::kStages;
-          ok = mbar_wait(&sh.p_ready, step & 1, abort_flag) &&
-               mbar_wait(&sh.full[stage], (n / C::kStages) & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          if (*reinterpret_cast<volatile int*>(&sh.keep_o)) {
-            fresh = false;
-            *reinterpret_cast<volatile int*>(&sh.keep_o) = 0;
-          }
-          const uint32_t vb = smem_u32(s_ring + stage * C::kTileBytes);
-#pragma unroll
-          for (int k = 0; k < kTile / 16; ++k) {
-            // V (keys x D) is MN-major: 64-column slabs 16 KiB apart, 8-key groups 1 KiB
-            umma_f16_ts(tmem + 128, tmem + 64 + k * 8,
-                        umma_smem_desc(vb + k * 2048, kTile * 128, 1024, 2), idesc_o,
-                        (k != 0 || !fresh) ? 1u : 0u);
-          }
-          umma_commit(&sh.empty[stage]);
-          ++n;
-          const bool block_end = it.left == 0;
-          if (block_end) umma_commit(&sh.o_full);
-          fresh = block_end;
-          t0 = next_step(p, list, pmax, it);
-        }
-        if (!ok) {
+      if (!ok) {
+        if (lane == 0) {
           *abort_flag = 1;
-          record_error(&g_error_word_tc, (kSiteMma << 8) | kErrReasonTimeout);
+          record_error(&g_error_word_tc, (kSiteProducer << 8) | kErrReasonTimeout);
         }
-        umma_commit(&sh.mma_done);  // every product is done before TMEM is given back
-        if (!mbar_wait(&sh.mma_done, 0, nullptr)) {
-          record_error(&g_error_word_tc, (kSiteDrain << 8) | kErrReasonTimeout);
+        sleep_ns(200000);  // the copies in flight land
+      }
+    } else if (warp == 9) {
+      // ---------------- tcgen05.mma ----------------
+      // The whole warp walks the steps, so that what it computes is uniform, and one lane
+      // issues; descriptors advance by constants.
+      constexpr uint32_t fmt = dtype_of<T>::value == 2 ? 1u : 0u;
+      constexpr uint32_t idesc_s = umma_idesc_f16(fmt, 0u, kTile, kTile);
+      constexpr uint32_t idesc_o = umma_idesc_f16(fmt, 1u, kTile, D);
+      constexpr uint64_t kTileUnits = C::kTileBytes >> 4;  // of descriptor addresses
+      const bool leader = elect_one();
+      const int steps0 = uniform(sh.item[0].steps), steps1 = uniform(sh.item[1].steps);
+      const bool both = __shfl_sync(0xffffffffu, shared, 0);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint64_t q_desc = umma_smem_desc(smem_u32(s_q), 16, 1024, 2);
+      const uint64_t k_desc = umma_smem_desc(smem_u32(s_ring), 16, 1024, 2);
+      // V (keys x D) is MN-major: 64-column slabs 16 KiB apart, 8-key groups 1 KiB
+      const uint64_t v_desc = umma_smem_desc(smem_u32(s_ring), kTile * 128, 1024, 2);
+      StepIter it0{uniform(sh.item[0].i0), 0, 0}, it1{uniform(sh.item[1].i0), 0, 0};
+      unsigned fresh = 3;  // bit k: item k's next product starts a key block
+      bool ok = true;
+      int stage = 0;       // of the next tile of the ring ...
+      uint32_t phase = 0;  // ... and its barrier's parity
+      int next = 0;        // and of the one behind it
+      uint32_t next_phase = 0;
+      auto behind = [&]() {
+        next = stage + 1;
+        next_phase = phase;
+        if (next == C::kStages) {
+          next = 0;
+          next_phase ^= 1u;
         }
+      };
+      auto advance = [&]() {
+        behind();
+        stage = next;
+        phase = next_phase;
+      };
+      const int rounds = max(steps0, steps1);
+      // Round j = -1: the first scores.  Round j: O += P V of each item's step j, then S = Q K^T
+      // of its step j + 1.
+#pragma unroll 1
+      for (int j = -1; j < rounds && ok; ++j) {
+#pragma unroll 1
+        for (int k = 0; k < 2 && ok; ++k) {
+          const int steps = k == 0 ? steps0 : steps1;
+          if (j >= steps || steps == 0) continue;
+          int ks = stage;
+          uint32_t kph = phase;
+          if (j < 0) {
+            ok = warp_wait(&sh.q_full[k], 0, abort_flag);
+          } else {
+            behind();
+            ks = next;
+            kph = next_phase;
+            StepIter it = k == 0 ? it0 : it1;
+            next_step(p, sh.item[k], it);
+            if (k == 0) it0 = it; else it1 = it;
+            const bool block_end = __shfl_sync(0xffffffffu, it.left == 0, 0);
+            ok = warp_wait(&sh.full[stage], phase, abort_flag) &&
+                 warp_wait(&sh.p_ready[k], j & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            volatile int* keep = &sh.keep_o[k];
+            bool first = (fresh >> k) & 1u;
+            if (uniform(*keep)) {
+              first = false;
+              __syncwarp();
+              if (leader) *keep = 0;
+            }
+            if (leader) {
+              const uint64_t vd = v_desc + stage * kTileUnits;
+              const uint32_t d = tm + 256 * k;
+              umma_f16_ts(d + 128, d + 64, vd, idesc_o, !first);
+#pragma unroll
+              for (int i = 1; i < kTile / 16; ++i) {
+                umma_f16_ts(d + 128, d + 64 + i * 8, vd + i * (2048 >> 4), idesc_o, true);
+              }
+              umma_commit(&sh.empty[stage]);
+              if (block_end) umma_commit(&sh.o_full[k]);
+            }
+            __syncwarp();
+            fresh = block_end ? fresh | (1u << k) : fresh & ~(1u << k);
+            if (!both) advance();  // (now the K tile, if there is one)
+          }
+          if (j + 1 < steps) {
+            ok = ok && warp_wait(&sh.full[ks], kph, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            if (leader) {
+              const uint64_t qd = q_desc + k * kTileUnits, kd = k_desc + ks * kTileUnits;
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i) {
+                const uint64_t off = ((i / 4) * (kTile * 128) + (i % 4) * 32) >> 4;
+                umma_f16(tm + 256 * k, qd + off, kd + off, idesc_s, i != 0 ? 1u : 0u);
+              }
+              umma_commit(&sh.empty[ks]);
+              umma_commit(&sh.s_full[k]);
+            }
+            __syncwarp();
+            if (!both) advance();
+          }
+        }
+        if (both) {  // V(j) and K(j + 1) served both items
+          advance();
+          if (j >= 0) advance();
+        }
+      }
+      if (!ok && leader) {
+        *abort_flag = 1;
+        record_error(&g_error_word_tc, (kSiteMma << 8) | kErrReasonTimeout);
+      }
+      __syncwarp();
+      if (leader) umma_commit(&sh.mma_done);  // every product is done before TMEM is given back
+      __syncwarp();
+      if (!warp_wait(&sh.mma_done, 0, nullptr) && leader) {
+        record_error(&g_error_word_tc, (kSiteDrain << 8) | kErrReasonTimeout);
       }
     }
   } else {
     // ---------------- softmax: thread = row ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-    const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
-    const uint32_t tS = tmem + lanes, tO = tmem + 128 + lanes;
-    const int row = warp * 32 + lane;
-    const bool live = row < rows;
-    const bool warp_live = warp * 32 < rows;
-    const int tok = row / p.G, head = w.kvh * p.G + (row - tok * p.G);
-    const int pos = live ? max(-1, pos0 + tok) : -1;
+    const int k = warp >> 2;
+    const Item& item = sh.item[k];
+    const int pieces = item.pieces, steps = item.steps;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t tS = tmem + 256 * k + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t tO = tS + 128;
+    const bool live = row < item.rows;
+    const bool warp_live = (warp & 3) * 32 < item.rows;
+    const int tok = p.by_head(row), head = item.kvh * p.G + (row - tok * p.G);
+    const int pos = live ? max(-1, item.pos0 + tok) : -1;
     const int lo_key = p.window == INT32_MAX ? 0 : pos - p.window + 1;  // of this row
     float tot_m = -INFINITY, tot_l = 0.f, tot_o[D];
 #pragma unroll
     for (int d = 0; d < D; ++d) tot_o[d] = 0.f;
     float m = -INFINITY, l = 0.f;
     bool fresh = true, ok = true;
-    int step = 0, block = 0;
-    StepIter it{i0, i1, 0, 0};
-    for (int t0 = next_step(p, list, pmax, it); t0 >= 0; ++step) {
+    int block = 0, scans = 0;
+    StepIter it{item.i0, 0, 0};
+    // do all rows see every key of the step at t0?
+    auto whole_for = [&](int t0, int pos0, int pmax) {
+      return t0 + kTile - 1 <= pos0 &&
+             (p.window == INT32_MAX || t0 > pmax - p.window || t0 + kTile <= p.first);
+    };
+    for (int step = 0; step < steps; ++step) {
+      const int t0 = next_step(p, item, it);
       const bool block_end = it.left == 0;
-      ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full, step & 1, abort_flag));
-      if (!ok) break;
-      tc_fence_after();
-      // does every row of the tile see every key of the step?
-      const bool whole = t0 + kTile - 1 <= pos0 &&
-                         (p.window == INT32_MAX || t0 > pmax - p.window ||
-                          t0 + kTile <= p.first);
+      const bool whole = whole_for(t0, item.pos0, item.pmax);
       uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
       if (!whole) {
 #pragma unroll
@@ -401,17 +576,32 @@ __global__ void __launch_bounds__(kThreads, 2)
           vis[b] = below(pos + 1 - k0) & (~below(lo_key - k0) | below(p.first - k0));
         }
       }
+      ok = warp_wait(&sh.s_full[k], step & 1, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      if (!whole && warp_live) {  // keys that the row does not see: a score of -inf
+#pragma unroll 1
+        for (int b = 0; b < 4; ++b) {
+          const uint32_t word = b == 0 ? vis[0] : b == 1 ? vis[1] : b == 2 ? vis[2] : vis[3];
+          uint32_t s[32];
+          tmem_ld_32x32b_x32(tS + 32 * b, s);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) s[j] = (word >> j) & 1u ? s[j] : 0xff800000u;
+          tmem_st_x32(tS + 32 * b, s);
+        }
+        tmem_st_wait();
+      }
       if (warp_live) {
         // The scores of keys 64..127 stay in registers from the maximum to the exponentials;
         // those of keys 0..63 are read twice.  P goes over the second half's scores: keys
         // 0..63 to columns 64..95, keys 64..127 to columns 96..127.
         uint32_t s[64];
         float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
+#pragma unroll 1
         for (int h = 0; h < 2; ++h) {
           tmem_ld_x64(tS + 64 * h, s);
           tmem_ld_wait();
-          if (!whole) mask_scores(s, vis[2 * h], vis[2 * h + 1]);
 #pragma unroll
           for (int j = 0; j < 64; j += 8) {
 #pragma unroll
@@ -428,12 +618,11 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (move) m = t;
         const float base = m == -INFINITY ? 0.f : -m;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+#pragma unroll 1
         for (int h = 1; h >= 0; --h) {
           if (h == 0) {
             tmem_ld_x64(tS, s);
             tmem_ld_wait();
-            if (!whole) mask_scores(s, vis[0], vis[1]);
           }
           uint32_t packed[32];
 #pragma unroll
@@ -461,20 +650,23 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         tmem_st_wait();
       }
-      if (!whole) {
-        // V of this step: thread = key
-        const int n = 2 * step + 1, stage = n % C::kStages;
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh.full[stage], (n / C::kStages) & 1, abort_flag));
+      if (!whole_for(t0, item.list_pos0, item.list_pmax)) {
+        // V of this step: thread = key (of shared tiles each item's threads take a half)
+        const int place = v_place(shared, sh.item[0].steps, sh.item[1].steps, k, step), stage = place % C::kStages;
+        ok = warp_wait(&sh.full[stage], (place / C::kStages) & 1, abort_flag);
         if (!ok) break;
         uint8_t* vrow = s_ring + stage * C::kTileBytes + row * 128;
         const int key = t0 + row;
-        const bool seen = key <= pmax && (key >= list.lo_key || key < p.first);
+        const bool seen = key <= item.list_pmax && (key >= item.list.lo_key || key < p.first);
         constexpr uint32_t em = exp_mask<T>();
-        bool bad = false;
+        constexpr int kChunks = C::kHalves * 8;
+        bool found = false;
+        const int c0 = shared ? k * (kChunks / 2) : 0;
+        const int c1 = shared ? c0 + kChunks / 2 : kChunks;
 #pragma unroll 1
-        for (int c = 0; c < C::kHalves * 8; ++c) {
+        for (int c = c0; c < c1; ++c) {
           uint4* at = reinterpret_cast<uint4*>(vrow + (c >> 3) * (kTile * 128) +
-                                               (((c + row) & 7) << 4));
+                                               (((c ^ row) & 7) << 4));
           uint4 x = *at;
           uint32_t* xw = reinterpret_cast<uint32_t*>(&x);
           bool hit = false;
@@ -490,13 +682,20 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
           }
           if (hit) *at = x;
-          bad |= hit;
+          found |= hit;
         }
-        const unsigned flags = __ballot_sync(0xffffffffu, bad && seen);
-        if (lane == 0) sh.bad[warp] = flags;
+        const unsigned flags = __ballot_sync(0xffffffffu, found && seen);
+        const int buf = scans++ & 1;
+        if (lane == 0) sh.bad[buf][k][warp & 3] = flags;
         fence_proxy_async_smem();  // the zeros, to the product's reads
-        softmax_sync();
-        if ((sh.bad[0] | sh.bad[1] | sh.bad[2] | sh.bad[3]) != 0) {
+        softmax_sync(k, shared);
+        unsigned bad[4], any = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          bad[b] = sh.bad[buf][k][b] | (shared ? sh.bad[buf][k ^ 1][b] : 0u);
+          any |= bad[b];
+        }
+        if (any != 0) {
           // add the non-finite values to the rows that see them
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
@@ -509,43 +708,46 @@ __global__ void __launch_bounds__(kThreads, 2)
               tmem_ld_wait();
             }
 #pragma unroll 1
-            for (int k = 0; k < kTile; ++k) {
-              if (((sh.bad[k >> 5] >> (k & 31)) & 1u) == 0) continue;
+            for (int i = 0; i < kTile; ++i) {
+              const uint32_t bw = i < 32 ? bad[0] : i < 64 ? bad[1] : i < 96 ? bad[2] : bad[3];
+              const uint32_t vw = i < 32 ? vis[0] : i < 64 ? vis[1] : i < 96 ? vis[2] : vis[3];
+              if (((bw >> (i & 31)) & 1u) == 0) continue;
               __syncwarp();
               uint32_t pw;
-              tmem_ld_x1(tS + 64 + (k >> 1), pw);
+              tmem_ld_x1(tS + 64 + (i >> 1), pw);
               tmem_ld_wait();
-              const float pk = unpack<T>(pw, k & 1);
-              const uint32_t word = k < 32 ? vis[0] : k < 64 ? vis[1] : k < 96 ? vis[2] : vis[3];
-              if (!live || ((word >> (k & 31)) & 1u) == 0) continue;
-              const int kk = t0 + k;
-              const int64_t pg = p.table[static_cast<int64_t>(w.r) * p.table_stride + kk / p.page];
-              const T* v = static_cast<const T*>(p.v) + pg * p.vs[0] + w.kvh * p.vs[1] +
-                           (kk % p.page) * p.vs[2] + c;
+              if (!live || ((vw >> (i & 31)) & 1u) == 0) continue;
+              const float pi = unpack<T>(pw, i & 1);
+              const int key_i = t0 + i;
+              const int col = p.by_page(key_i);
+              const int64_t pg = p.table[static_cast<int64_t>(item.r) * p.table_stride + col];
+              const T* v = static_cast<const T*>(p.v) + pg * p.vs[0] + item.kvh * p.vs[1] +
+                           (key_i - col * p.page) * p.vs[2] + c;
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
                 const float x = to_f32(v[j]);
-                if (!isfinite(x)) o[j] = __float_as_uint(__uint_as_float(o[j]) + pk * x);
+                if (!isfinite(x)) o[j] = __float_as_uint(__uint_as_float(o[j]) + pi * x);
               }
             }
             __syncwarp();
             tmem_st_x32(tO + c, o);
           }
           tmem_st_wait();
-          if (tid == 0) *reinterpret_cast<volatile int*>(&sh.keep_o) = 1;
+          if (row == 0) *const_cast<volatile int*>(&sh.keep_o[k]) = 1;
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.p_ready);
+      if (lane == 0) mbar_arrive(&sh.p_ready[k]);
       fresh = false;
       if (block_end) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full, block & 1, abort_flag));
+        ok = warp_wait(&sh.o_full[k], block & 1, abort_flag);
         if (!ok) break;
         tc_fence_after();
         if (warp_live) {
-          if (w.pieces > 1) {
-            const int64_t at = part_slot(p, w.base, w.blocks, tok0 + tok, head, i0 + block);
+          if (pieces > 1) {
+            const int64_t at = part_slot(p, item.base, item.blocks, item.tok0 + tok, head,
+                                         item.i0 + block);
             if (live) p.part_ml[at] = make_float2(m, l);
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
@@ -583,20 +785,17 @@ __global__ void __launch_bounds__(kThreads, 2)
         fresh = true;
         ++block;
       }
-      t0 = next_step(p, list, pmax, it);
     }
     if (!ok) {
       if (lane == 0) {
         *abort_flag = 1;
         record_error(&g_error_word_tc, (kSiteSoftmax << 8) | kErrReasonTimeout);
       }
-    } else if (w.pieces == 1 && live) {
+    } else if (pieces == 1 && live) {
       const float sink = p.sinks ? to_f32(static_cast<const T*>(p.sinks)[head]) * kLog2e : 0.f;
       const float sc = row_scale(tot_m, tot_l, p.sinks != nullptr, sink);
-      T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(w.x.tok + tok0 + tok) * p.os[0] +
+      T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(item.tok + tok) * p.os[0] +
                head * p.os[1];
-      const bool vec = (p.os[0] % 8 | p.os[1] % 8) == 0 &&
-                       (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
 #pragma unroll
       for (int d = 0; d < D; d += 8) {
         uint32_t x[4];
@@ -604,15 +803,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int j = 0; j < 4; ++j) {
           x[j] = pack2<T>(row_value(tot_o[d + 2 * j], sc), row_value(tot_o[d + 2 * j + 1], sc));
         }
-        if (vec) {
-          *reinterpret_cast<uint4*>(dst + d) = make_uint4(x[0], x[1], x[2], x[3]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint16_t h = static_cast<uint16_t>(j & 1 ? x[j / 2] >> 16 : x[j / 2] & 0xffffu);
-            dst[d + j] = *reinterpret_cast<const T*>(&h);
-          }
-        }
+        *reinterpret_cast<uint4*>(dst + d) = make_uint4(x[0], x[1], x[2], x[3]);
       }
     }
   }
@@ -620,7 +811,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 5) {
+  if (warp == 9) {
     __syncwarp();
     tmem_dealloc(tmem, kTmemCols);
   }
@@ -653,7 +844,7 @@ static int launch(const PagedSdpaArgs& a, const Params& p, int64_t items, cudaSt
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(paged_sdpa)");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(items));
+  cfg.gridDim = dim3(static_cast<unsigned>((items + 1) / 2));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = stream;

@@ -296,6 +296,13 @@ def _attention_eager(q, k_cache, v_cache, block_table, query_start, seq_lens, sc
     if (q.data_ptr() % 16 or q.stride(2) != 1
             or any((s % vec or s == 0) and n > 1 for s, n in zip(q.stride()[:2], q.shape[:2]))):
         q = q.contiguous() if not q.is_contiguous() else q.clone()
+    if out.data_ptr() % 16 or any(s % vec for s in out.stride()[:2]):
+        # the kernels store 16-byte vectors: go through an aligned copy (rows outside every
+        # request come back as they were)
+        tmp = _attention_eager(q, k_cache, v_cache, block_table, query_start, seq_lens, scale,
+                               window, first_tokens, sinks, out.clone(
+                                   memory_format=torch.contiguous_format), code, dev)
+        return out.copy_(tmp)
     lib = _lib.lib()
     with torch.cuda.device(dev):
         ws = torch.empty(lib.bi_paged_sdpa_workspace(T, R, H, D, width, page),
