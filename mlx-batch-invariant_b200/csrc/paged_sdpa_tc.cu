@@ -33,8 +33,8 @@ namespace tcp {
 
 constexpr int kThreads = 384;
 constexpr int kTile = 128;            // rows of a tile and keys of a step
-constexpr int kRegsSoftmax = 216;     // 2 x 216 + 72 = 3 x 168, the launch's registers
-constexpr int kRegsOther = 72;
+constexpr int kRegsSoftmax = 224;     // 2 x 224 + 56 = 3 x 168, the launch's registers
+constexpr int kRegsOther = 56;
 constexpr int kTmemCols = 512;        // per item: S (P over its second half) and O, 128 each
 constexpr float kSlack = 8.f;         // log 2 of how far weights may exceed 1
 constexpr int kMaxStages = 12;
@@ -55,25 +55,27 @@ __device__ __forceinline__ void tmem_ld_x1(uint32_t taddr, uint32_t& r) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr)
                : "memory");
 }
-__device__ __forceinline__ void tmem_ld_x64(uint32_t taddr, uint32_t (&r)[64]) {
+// Waits for this warp's TMEM loads; the registers pass through, so that nothing that uses them
+// is moved ahead of the wait.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+        "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+        "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+        "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+      :
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait1(uint32_t& r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r) : : "memory");
+}
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
-      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, "
-      "%35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, "
-      "%52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
-        "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
-        "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
-        "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
-        "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
-        "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]),
-        "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]),
-        "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]),
-        "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-      : "r"(taddr)
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -155,6 +157,20 @@ __device__ __forceinline__ void fma2(float& x0, float& x1, float a, float b) {  
       "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
       : "+f"(x0), "+f"(x1) : "f"(a), "f"(b));
 }
+__device__ __forceinline__ void mul2(float& x0, float& x1, float a) {
+  asm("{\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(x0), "+f"(x1) : "f"(a));
+}
+// x = y b + x a, the product x a rounded first
+__device__ __forceinline__ void fold2(float& x0, float& x1, float y0, float y1, float a, float b) {
+  asm("{\n\t.reg .b64 x, y, u, v;\n\t"
+      "mov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
+      "mov.b64 u, {%4, %4};\n\tmov.b64 v, {%5, %5};\n\t"
+      "mul.rn.f32x2 x, x, u;\n\tfma.rn.f32x2 x, y, v, x;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(x0), "+f"(x1) : "f"(y0), "f"(y1), "f"(a), "f"(b));
+}
 __device__ __forceinline__ void add2(float& x0, float& x1, float y0, float y1) {
   asm("{\n\t.reg .b64 x, y;\n\t"
       "mov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
@@ -181,6 +197,34 @@ __device__ __forceinline__ float unpack(uint32_t w, int hi) {
 template <typename T>
 __device__ __forceinline__ constexpr uint32_t exp_mask() {
   return dtype_of<T>::value == 2 ? 0x7f80u : 0x7c00u;
+}
+
+// The larger of `top` and 32 scores, in four chains.
+__device__ __forceinline__ void max_of(const uint32_t (&s)[32], float (&tops)[4]) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 8) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      tops[c] = fmaxf(tops[c], fmaxf(__uint_as_float(s[j + 2 * c]),
+                                     __uint_as_float(s[j + 2 * c + 1])));
+    }
+  }
+}
+// The weights 2^(s scale + base) of 32 scores: added to `sum`, and rounded to T in TMEM.
+template <typename T>
+__device__ __forceinline__ void weights_of(const uint32_t (&s)[32], float scale, float base,
+                                           float (&sum)[4], uint32_t taddr) {
+  uint32_t packed[16];
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    float x0 = __uint_as_float(s[j]), x1 = __uint_as_float(s[j + 1]);
+    fma2(x0, x1, scale, base);
+    x0 = exp2_approx(x0);
+    x1 = exp2_approx(x1);
+    add2(sum[j % 4], sum[j % 4 + 1], x0, x1);
+    packed[j / 2] = pack2<T>(x0, x1);
+  }
+  tmem_st_x16(taddr, packed);
 }
 
 // What one of a block's two items is.
@@ -279,8 +323,8 @@ __device__ __forceinline__ int v_place(bool shared, int l0, int l1, int k, int j
 
 struct Shared {
   SchedSmem<kThreads, 2> sched;
-  uint64_t q_full[2], full[kMaxStages], empty[kMaxStages], s_full[2], p_ready[2], o_full[2],
-      mma_done;
+  uint64_t q_full[2], full[kMaxStages], empty[kMaxStages], s_full[2], p_half[2], p_ready[2],
+      o_full[2], mma_done;
   uint32_t tmem;
   int abort_flag;
   Item item[2];
@@ -324,6 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int k = 0; k < 2; ++k) {
       mbar_init(&sh.q_full[k], 1);
       mbar_init(&sh.s_full[k], 1);
+      mbar_init(&sh.p_half[k], 4);
       mbar_init(&sh.p_ready[k], 4);
       mbar_init(&sh.o_full[k], 1);
       sh.keep_o[k] = 0;
@@ -466,6 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (j >= steps || steps == 0) continue;
           int ks = stage;
           uint32_t kph = phase;
+          bool ends = false;  // the step ends its key block
           if (j < 0) {
             ok = warp_wait(&sh.q_full[k], 0, abort_flag);
           } else {
@@ -475,9 +521,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             StepIter it = k == 0 ? it0 : it1;
             next_step(p, sh.item[k], it);
             if (k == 0) it0 = it; else it1 = it;
-            const bool block_end = __shfl_sync(0xffffffffu, it.left == 0, 0);
-            ok = warp_wait(&sh.full[stage], phase, abort_flag) &&
-                 warp_wait(&sh.p_ready[k], j & 1, abort_flag);
+            ends = __shfl_sync(0xffffffffu, it.left == 0, 0);
+            ok = warp_wait(&sh.full[stage], phase, abort_flag);
+          }
+          if (j + 1 < steps) ok = ok && warp_wait(&sh.full[ks], kph, abort_flag);
+          if (j >= 0) {
+            ok = ok && warp_wait(&sh.p_half[k], j & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
             volatile int* keep = &sh.keep_o[k];
@@ -487,25 +536,35 @@ __global__ void __launch_bounds__(kThreads, 1)
               __syncwarp();
               if (leader) *keep = 0;
             }
+            // keys 64..127 while the weights of keys 0..63 are still being computed
+            const uint64_t vd = v_desc + stage * kTileUnits;
+            const uint32_t d = tm + 256 * k;
             if (leader) {
-              const uint64_t vd = v_desc + stage * kTileUnits;
-              const uint32_t d = tm + 256 * k;
-              umma_f16_ts(d + 128, d + 64, vd, idesc_o, !first);
+              umma_f16_ts(d + 128, d + 64 + 4 * 8, vd + 4 * (2048 >> 4), idesc_o, !first);
 #pragma unroll
-              for (int i = 1; i < kTile / 16; ++i) {
+              for (int i = 5; i < 8; ++i) {
+                umma_f16_ts(d + 128, d + 64 + i * 8, vd + i * (2048 >> 4), idesc_o, true);
+              }
+            }
+            __syncwarp();
+            ok = warp_wait(&sh.p_ready[k], j & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            if (leader) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
                 umma_f16_ts(d + 128, d + 64 + i * 8, vd + i * (2048 >> 4), idesc_o, true);
               }
               umma_commit(&sh.empty[stage]);
-              if (block_end) umma_commit(&sh.o_full[k]);
+              if (j + 1 == steps) umma_commit(&sh.o_full[k]);
             }
             __syncwarp();
-            fresh = block_end ? fresh | (1u << k) : fresh & ~(1u << k);
+            fresh = ends ? fresh | (1u << k) : fresh & ~(1u << k);
             if (!both) advance();  // (now the K tile, if there is one)
           }
+          if (!ok) break;
           if (j + 1 < steps) {
-            ok = ok && warp_wait(&sh.full[ks], kph, abort_flag);
-            if (!ok) break;
-            tc_fence_after();
+            if (j < 0) tc_fence_after();
             if (leader) {
               const uint64_t qd = q_desc + k * kTileUnits, kd = k_desc + ks * kTileUnits;
 #pragma unroll
@@ -554,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
     for (int d = 0; d < D; ++d) tot_o[d] = 0.f;
     float m = -INFINITY, l = 0.f;
-    bool fresh = true, ok = true;
+    bool fresh = true, ok = true;  // fresh: the step starts a key block
     int block = 0, scans = 0;
     StepIter it{item.i0, 0, 0};
     // do all rows see every key of the step at t0?
@@ -562,10 +621,49 @@ __global__ void __launch_bounds__(kThreads, 1)
       return t0 + kTile - 1 <= pos0 &&
              (p.window == INT32_MAX || t0 > pmax - p.window || t0 + kTile <= p.first);
     };
+    // The finished key block's O, with its (bm, bl): joined to the running result, or (split
+    // items) left for the join.
+    auto close_block = [&](float bm, float bl) {
+      if (pieces > 1) {
+        const int64_t at = part_slot(p, item.base, item.blocks, item.tok0 + tok, head,
+                                     item.i0 + block);
+        if (live) p.part_ml[at] = make_float2(bm, bl);
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(tO + c, o);
+          tmem_ld_wait(o);
+          if (live) {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + c);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              dst[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]),
+                                   __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
+            }
+          }
+        }
+      } else {
+        float fa, fb;
+        fold_factors(tot_m, bm, fa, fb);
+        tot_l = fold_value(tot_l, bl, fa, fb);
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(tO + c, o);
+          tmem_ld_wait(o);
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            fold2(tot_o[c + j], tot_o[c + j + 1], __uint_as_float(o[j]),
+                  __uint_as_float(o[j + 1]), fa, fb);
+          }
+        }
+      }
+      ++block;
+    };
     for (int step = 0; step < steps; ++step) {
       const int t0 = next_step(p, item, it);
-      const bool block_end = it.left == 0;
       const bool whole = whole_for(t0, item.pos0, item.pmax);
+      const bool list_whole = whole_for(t0, item.list_pos0, item.list_pmax);
       uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
       if (!whole) {
 #pragma unroll
@@ -576,83 +674,85 @@ __global__ void __launch_bounds__(kThreads, 1)
           vis[b] = below(pos + 1 - k0) & (~below(lo_key - k0) | below(p.first - k0));
         }
       }
+      // S of this step; with it the product before it in the queue, the last step's P V, is done
       ok = warp_wait(&sh.s_full[k], step & 1, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      if (!whole && warp_live) {  // keys that the row does not see: a score of -inf
-#pragma unroll 1
-        for (int b = 0; b < 4; ++b) {
-          const uint32_t word = b == 0 ? vis[0] : b == 1 ? vis[1] : b == 2 ? vis[2] : vis[3];
-          uint32_t s[32];
-          tmem_ld_32x32b_x32(tS + 32 * b, s);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) s[j] = (word >> j) & 1u ? s[j] : 0xff800000u;
-          tmem_st_x32(tS + 32 * b, s);
-        }
-        tmem_st_wait();
-      }
+      uint32_t sa[32], sb[32];
+      // keys 64..127 again, behind work that needs the registers
+      auto reload = [&]() {
+        tmem_ld_32x32b_x32(tS + 64, sa);
+        tmem_ld_32x32b_x32(tS + 96, sb);
+        tmem_ld_wait(sa);
+        tmem_ld_wait(sb);
+      };
+      float base = 0.f, f = 1.f;
       if (warp_live) {
+        if (!whole) {  // keys that the row does not see: a score of -inf
+#pragma unroll 1
+          for (int b = 0; b < 4; ++b) {
+            const uint32_t word = b == 0 ? vis[0] : b == 1 ? vis[1] : b == 2 ? vis[2] : vis[3];
+            tmem_ld_32x32b_x32(tS + 32 * b, sa);
+            tmem_ld_wait(sa);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sa[j] = (word >> j) & 1u ? sa[j] : 0xff800000u;
+            tmem_st_x32(tS + 32 * b, sa);
+          }
+          tmem_st_wait();
+        }
         // The scores of keys 64..127 stay in registers from the maximum to the exponentials;
         // those of keys 0..63 are read twice.  P goes over the second half's scores: keys
         // 0..63 to columns 64..95, keys 64..127 to columns 96..127.
-        uint32_t s[64];
         float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
-          tmem_ld_x64(tS + 64 * h, s);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 64; j += 8) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              tops[c] = fmaxf(tops[c], fmaxf(__uint_as_float(s[j + 2 * c]),
-                                             __uint_as_float(s[j + 2 * c + 1])));
-            }
-          }
+          tmem_ld_32x32b_x32(tS + 64 * h, sa);
+          tmem_ld_32x32b_x32(tS + 64 * h + 32, sb);
+          tmem_ld_wait(sa);
+          tmem_ld_wait(sb);
+          max_of(sa, tops);
+          max_of(sb, tops);
         }
         const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         const float t = top == -INFINITY ? top : top * p.scale_log2;
-        const bool move = t > m + kSlack;  // (also from m = -inf)
-        const float f = move ? exp2_approx(m - t) : 1.f;
-        if (move) m = t;
-        const float base = m == -INFINITY ? 0.f : -m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-        for (int h = 1; h >= 0; --h) {
-          if (h == 0) {
-            tmem_ld_x64(tS, s);
-            tmem_ld_wait();
+        if (fresh) {
+          const float bm = m, bl = l;
+          m = t;
+          l = 0.f;
+          if (step > 0) {
+            close_block(bm, bl);
+            reload();
           }
-          uint32_t packed[32];
-#pragma unroll
-          for (int j = 0; j < 64; j += 2) {
-            float x0 = __uint_as_float(s[j]), x1 = __uint_as_float(s[j + 1]);
-            fma2(x0, x1, p.scale_log2, base);
-            x0 = exp2_approx(x0);
-            x1 = exp2_approx(x1);
-            add2(sum[j % 4], sum[j % 4 + 1], x0, x1);
-            packed[j / 2] = pack2<T>(x0, x1);
+        } else {
+          const bool move = t > m + kSlack;  // (also from m = -inf)
+          if (move) {
+            f = exp2_approx(m - t);
+            m = t;
           }
-          tmem_st_x32(tS + 64 + 32 * h, packed);
-        }
-        l = __fmaf_rn(l, f, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
-        if (!fresh && __any_sync(0xffffffffu, move)) {
+          if (__any_sync(0xffffffffu, move)) {
 #pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            uint32_t o[32];
-            tmem_ld_32x32b_x32(tO + c, o);
-            tmem_ld_wait();
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(tO + c, o);
+              tmem_ld_wait(o);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__fmul_rn(__uint_as_float(o[j]), f));
-            tmem_st_x32(tO + c, o);
+              for (int j = 0; j < 32; j += 2) {
+                float x0 = __uint_as_float(o[j]), x1 = __uint_as_float(o[j + 1]);
+                mul2(x0, x1, f);
+                o[j] = __float_as_uint(x0);
+                o[j + 1] = __float_as_uint(x1);
+              }
+              tmem_st_x32(tO + c, o);
+            }
+            reload();
           }
         }
-        tmem_st_wait();
+        base = m == -INFINITY ? 0.f : -m;
       }
-      if (!whole_for(t0, item.list_pos0, item.list_pmax)) {
+      if (!list_whole) {
         // V of this step: thread = key (of shared tiles each item's threads take a half)
-        const int place = v_place(shared, sh.item[0].steps, sh.item[1].steps, k, step), stage = place % C::kStages;
+        const int place = v_place(shared, sh.item[0].steps, sh.item[1].steps, k, step);
+        const int stage = place % C::kStages;
         ok = warp_wait(&sh.full[stage], (place / C::kStages) & 1, abort_flag);
         if (!ok) break;
         uint8_t* vrow = s_ring + stage * C::kTileBytes + row * 128;
@@ -705,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int j = 0; j < 32; ++j) o[j] = 0u;
             } else {
               tmem_ld_32x32b_x32(tO + c, o);
-              tmem_ld_wait();
+              tmem_ld_wait(o);
             }
 #pragma unroll 1
             for (int i = 0; i < kTile; ++i) {
@@ -713,11 +813,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               const uint32_t vw = i < 32 ? vis[0] : i < 64 ? vis[1] : i < 96 ? vis[2] : vis[3];
               if (((bw >> (i & 31)) & 1u) == 0) continue;
               __syncwarp();
-              uint32_t pw;
-              tmem_ld_x1(tS + 64 + (i >> 1), pw);
-              tmem_ld_wait();
+              uint32_t score;
+              tmem_ld_x1(tS + i, score);
+              tmem_ld_wait1(score);
               if (!live || ((vw >> (i & 31)) & 1u) == 0) continue;
-              const float pi = unpack<T>(pw, i & 1);
+              const float x = exp2_approx(__fmaf_rn(__uint_as_float(score), p.scale_log2, base));
+              const float pi = unpack<T>(pack2<T>(x, x), 0);
               const int key_i = t0 + i;
               const int col = p.by_page(key_i);
               const int64_t pg = p.table[static_cast<int64_t>(item.r) * p.table_stride + col];
@@ -725,66 +826,45 @@ __global__ void __launch_bounds__(kThreads, 1)
                            (key_i - col * p.page) * p.vs[2] + c;
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
-                const float x = to_f32(v[j]);
-                if (!isfinite(x)) o[j] = __float_as_uint(__uint_as_float(o[j]) + pi * x);
+                const float y = to_f32(v[j]);
+                if (!isfinite(y)) o[j] = __float_as_uint(__uint_as_float(o[j]) + pi * y);
               }
             }
             __syncwarp();
             tmem_st_x32(tO + c, o);
           }
-          tmem_st_wait();
           if (row == 0) *const_cast<volatile int*>(&sh.keep_o[k]) = 1;
         }
+        reload();
       }
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      if (warp_live) {
+        weights_of<T>(sa, p.scale_log2, base, sum, tS + 96);
+        tmem_ld_32x32b_x32(tS, sa);
+        weights_of<T>(sb, p.scale_log2, base, sum, tS + 112);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.p_half[k]);
+      if (warp_live) {
+        tmem_ld_wait(sa);
+        tmem_ld_32x32b_x32(tS + 32, sb);
+        weights_of<T>(sa, p.scale_log2, base, sum, tS + 64);
+        tmem_ld_wait(sb);
+        weights_of<T>(sb, p.scale_log2, base, sum, tS + 80);
+      }
+      tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.p_ready[k]);
-      fresh = false;
-      if (block_end) {
-        ok = warp_wait(&sh.o_full[k], block & 1, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        if (warp_live) {
-          if (pieces > 1) {
-            const int64_t at = part_slot(p, item.base, item.blocks, item.tok0 + tok, head,
-                                         item.i0 + block);
-            if (live) p.part_ml[at] = make_float2(m, l);
-#pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_ld_32x32b_x32(tO + c, o);
-              tmem_ld_wait();
-              if (live) {
-                float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + c);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  dst[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]),
-                                       __uint_as_float(o[4 * j + 2]),
-                                       __uint_as_float(o[4 * j + 3]));
-                }
-              }
-            }
-          } else {
-            float fa, fb;
-            fold_factors(tot_m, m, fa, fb);
-            tot_l = fold_value(tot_l, l, fa, fb);
-#pragma unroll
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_ld_32x32b_x32(tO + c, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                tot_o[c + j] = fold_value(tot_o[c + j], __uint_as_float(o[j]), fa, fb);
-              }
-            }
-          }
-        }
-        m = -INFINITY;
-        l = 0.f;
-        fresh = true;
-        ++block;
-      }
+      l = __fmaf_rn(l, f, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
+      fresh = it.left == 0;
+    }
+    if (ok && steps > 0) {
+      ok = warp_wait(&sh.o_full[k], 0, abort_flag);
+      tc_fence_after();
+      if (ok && warp_live) close_block(m, l);
     }
     if (!ok) {
       if (lane == 0) {
