@@ -150,32 +150,31 @@ __device__ __forceinline__ void softmax_sync(int item, bool both) {
   }
 }
 
-// Two fp32 operations in one instruction, each rounded to nearest.
-__device__ __forceinline__ void fma2(float& x0, float& x1, float a, float b) {  // x a + b
-  asm("{\n\t.reg .b64 x, y, z;\n\t"
-      "mov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\tmov.b64 z, {%3, %3};\n\t"
-      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "+f"(x0), "+f"(x1) : "f"(a), "f"(b));
+// Two fp32 numbers in one 64-bit register, two operations in one instruction, each rounded to
+// nearest.  (Constants are kept packed: a register short, the compiler would otherwise pack
+// them anew at every use.)
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
 }
-__device__ __forceinline__ void mul2(float& x0, float& x1, float a) {
-  asm("{\n\t.reg .b64 x, y;\n\t"
-      "mov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\t"
-      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "+f"(x0), "+f"(x1) : "f"(a));
+__device__ __forceinline__ void unpair(uint64_t x, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x));
 }
-// x = y b + x a, the product x a rounded first
-__device__ __forceinline__ void fold2(float& x0, float& x1, float y0, float y1, float a, float b) {
-  asm("{\n\t.reg .b64 x, y, u, v;\n\t"
-      "mov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
-      "mov.b64 u, {%4, %4};\n\tmov.b64 v, {%5, %5};\n\t"
-      "mul.rn.f32x2 x, x, u;\n\tfma.rn.f32x2 x, y, v, x;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "+f"(x0), "+f"(x1) : "f"(y0), "f"(y1), "f"(a), "f"(b));
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
 }
-__device__ __forceinline__ void add2(float& x0, float& x1, float y0, float y1) {
-  asm("{\n\t.reg .b64 x, y;\n\t"
-      "mov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
-      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "+f"(x0), "+f"(x1) : "f"(y0), "f"(y1));
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
 }
 
 template <typename T>
@@ -212,16 +211,16 @@ __device__ __forceinline__ void max_of(const uint32_t (&s)[32], float (&tops)[4]
 }
 // The weights 2^(s scale + base) of 32 scores: added to `sum`, and rounded to T in TMEM.
 template <typename T>
-__device__ __forceinline__ void weights_of(const uint32_t (&s)[32], float scale, float base,
-                                           float (&sum)[4], uint32_t taddr) {
+__device__ __forceinline__ void weights_of(const uint32_t (&s)[32], uint64_t scale, uint64_t base,
+                                           uint64_t (&sum)[2], uint32_t taddr) {
   uint32_t packed[16];
 #pragma unroll
   for (int j = 0; j < 32; j += 2) {
-    float x0 = __uint_as_float(s[j]), x1 = __uint_as_float(s[j + 1]);
-    fma2(x0, x1, scale, base);
+    float x0, x1;
+    unpair(fma2(pair(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), scale, base), x0, x1);
     x0 = exp2_approx(x0);
     x1 = exp2_approx(x1);
-    add2(sum[j % 4], sum[j % 4 + 1], x0, x1);
+    sum[(j / 2) % 2] = add2(sum[(j / 2) % 2], pair(x0, x1));
     packed[j / 2] = pack2<T>(x0, x1);
   }
   tmem_st_x16(taddr, packed);
@@ -609,9 +608,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int tok = p.by_head(row), head = item.kvh * p.G + (row - tok * p.G);
     const int pos = live ? max(-1, item.pos0 + tok) : -1;
     const int lo_key = p.window == INT32_MAX ? 0 : pos - p.window + 1;  // of this row
-    float tot_m = -INFINITY, tot_l = 0.f, tot_o[D];
+    float tot_m = -INFINITY, tot_l = 0.f;
+    uint64_t tot_o[D / 2];
 #pragma unroll
-    for (int d = 0; d < D; ++d) tot_o[d] = 0.f;
+    for (int d = 0; d < D / 2; ++d) tot_o[d] = 0ull;
+    const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
     float m = -INFINITY, l = 0.f;
     bool fresh = true, ok = true;  // fresh: the step starts a key block
     int block = 0, scans = 0;
@@ -646,15 +647,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         float fa, fb;
         fold_factors(tot_m, bm, fa, fb);
         tot_l = fold_value(tot_l, bl, fa, fb);
+        const uint64_t fa2 = pair(fa, fa), fb2 = pair(fb, fb);
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
           uint32_t o[32];
           tmem_ld_32x32b_x32(tO + c, o);
           tmem_ld_wait(o);
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            fold2(tot_o[c + j], tot_o[c + j + 1], __uint_as_float(o[j]),
-                  __uint_as_float(o[j + 1]), fa, fb);
+          for (int j = 0; j < 32; j += 2) {  // fold_value, two at a time
+            uint64_t& x = tot_o[(c + j) / 2];
+            x = fma2(pair(__uint_as_float(o[j]), __uint_as_float(o[j + 1])), fb2, mul2(x, fa2));
           }
         }
       }
@@ -688,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       float base = 0.f, f = 1.f;
       if (warp_live) {
-        if (!whole) {  // keys that the row does not see: a score of -inf
+        if (__builtin_expect(!whole, 0)) {  // keys that the row does not see: a score of -inf
 #pragma unroll 1
           for (int b = 0; b < 4; ++b) {
             const uint32_t word = b == 0 ? vis[0] : b == 1 ? vis[1] : b == 2 ? vis[2] : vis[3];
@@ -729,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             f = exp2_approx(m - t);
             m = t;
           }
-          if (__any_sync(0xffffffffu, move)) {
+          if (__builtin_expect(__any_sync(0xffffffffu, move), 0)) {
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
               uint32_t o[32];
@@ -737,8 +739,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_ld_wait(o);
 #pragma unroll
               for (int j = 0; j < 32; j += 2) {
-                float x0 = __uint_as_float(o[j]), x1 = __uint_as_float(o[j + 1]);
-                mul2(x0, x1, f);
+                float x0, x1;
+                unpair(mul2(pair(__uint_as_float(o[j]), __uint_as_float(o[j + 1])), pair(f, f)), x0,
+                       x1);
                 o[j] = __float_as_uint(x0);
                 o[j + 1] = __float_as_uint(x1);
               }
@@ -749,7 +752,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         base = m == -INFINITY ? 0.f : -m;
       }
-      if (!list_whole) {
+      if (__builtin_expect(!list_whole, 0)) {
         // V of this step: thread = key (of shared tiles each item's threads take a half)
         const int place = v_place(shared, sh.item[0].steps, sh.item[1].steps, k, step);
         const int stage = place % C::kStages;
@@ -795,7 +798,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           bad[b] = sh.bad[buf][k][b] | (shared ? sh.bad[buf][k ^ 1][b] : 0u);
           any |= bad[b];
         }
-        if (any != 0) {
+        if (__builtin_expect(any != 0, 0)) {
           // add the non-finite values to the rows that see them
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
@@ -837,11 +840,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         reload();
       }
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      uint64_t sum[2] = {0ull, 0ull};
+      const uint64_t base2 = pair(base, base);
       if (warp_live) {
-        weights_of<T>(sa, p.scale_log2, base, sum, tS + 96);
+        weights_of<T>(sa, scale2, base2, sum, tS + 96);
         tmem_ld_32x32b_x32(tS, sa);
-        weights_of<T>(sb, p.scale_log2, base, sum, tS + 112);
+        weights_of<T>(sb, scale2, base2, sum, tS + 112);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -850,15 +854,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (warp_live) {
         tmem_ld_wait(sa);
         tmem_ld_32x32b_x32(tS + 32, sb);
-        weights_of<T>(sa, p.scale_log2, base, sum, tS + 64);
+        weights_of<T>(sa, scale2, base2, sum, tS + 64);
         tmem_ld_wait(sb);
-        weights_of<T>(sb, p.scale_log2, base, sum, tS + 80);
+        weights_of<T>(sb, scale2, base2, sum, tS + 80);
       }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.p_ready[k]);
-      l = __fmaf_rn(l, f, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
+      float s0, s1;
+      unpair(add2(sum[0], sum[1]), s0, s1);
+      l = __fmaf_rn(l, f, __fadd_rn(s0, s1));
       fresh = it.left == 0;
     }
     if (ok && steps > 0) {
@@ -881,7 +887,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t x[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          x[j] = pack2<T>(row_value(tot_o[d + 2 * j], sc), row_value(tot_o[d + 2 * j + 1], sc));
+          float o0, o1;
+          unpair(tot_o[d / 2 + j], o0, o1);
+          x[j] = pack2<T>(row_value(o0, sc), row_value(o1, sc));
         }
         *reinterpret_cast<uint4*>(dst + d) = make_uint4(x[0], x[1], x[2], x[3]);
       }
