@@ -1,10 +1,11 @@
-"""Builds libbi.so (the C-ABI kernel library) in-tree for sm_100a with nvcc.
+"""Builds libbi.so (the C-ABI kernel library) in-tree for sm_100a with nvcc, and _bind.so (the
+short way to its paged-cache operators from Python) with g++.
 
     python mlx-batch-invariant_b200/build.py [--force] [-j N]
 
 Objects go to mlx-batch-invariant_b200/_build/, the library to
 mlx-batch-invariant_b200/mlx_batch_invariant_b200/libbi.so, where the Python
-package loads it.  A source is recompiled only when it, or a header, is newer
+package loads it; _bind.so goes beside it.  A source is recompiled only when it, or a header, is newer
 than its object.
 """
 
@@ -14,12 +15,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "mlx_batch_invariant_b200", "libbi.so")
+BIND = os.path.join(HERE, "mlx_batch_invariant_b200", "_bind.so")
 INCLUDE = os.path.join(ROOT, "include")
 
 SOURCES = ["capi.cu", "gemm_tcgen05.cu", "gemm_tf32x3.cu", "gemm_simt.cu", "sdpa.cu",
@@ -58,8 +61,40 @@ def _compile(src, extra):
     return obj, r.stderr
 
 
+def _cuda_include():
+    return os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
+
+
+def build_bind(force=False):
+    """The CPython module over torch's C++ headers (no pybind, no JIT cache)."""
+    src = os.path.join(CSRC, "bind.cpp")
+    if not (force or _stale(BIND, [src, os.path.join(INCLUDE, "bi.h")])):
+        return BIND
+    import torch
+    base = os.path.dirname(os.path.abspath(torch.__file__))
+    inc = os.path.join(base, "include")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+           "-I" + INCLUDE, "-I" + inc, "-I" + os.path.join(inc, "torch", "csrc", "api", "include"),
+           "-I" + sysconfig.get_paths()["include"], "-I" + _cuda_include(), src, "-o", BIND,
+           "-L" + os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu",
+           "-lc10_cuda", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed on bind.cpp:\n%s\n%s" % (" ".join(cmd), r.stderr))
+    return BIND
+
+
 def build(force=False, jobs=None, verbose=False, extra=()):
     os.makedirs(BUILD, exist_ok=True)
+    with concurrent.futures.ThreadPoolExecutor(max_workers=1) as side:
+        bind = side.submit(build_bind, force)
+        lib = _build_lib(force, jobs, verbose, extra)
+        bind.result()
+    return lib
+
+
+def _build_lib(force, jobs, verbose, extra):
     headers = _headers()
     srcs = [os.path.join(CSRC, s) for s in SOURCES]
     objs = [os.path.join(BUILD, s.replace(".cu", ".o")) for s in SOURCES]

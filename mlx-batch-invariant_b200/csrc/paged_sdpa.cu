@@ -10,15 +10,28 @@ namespace psdpa {
 
 // ---------------------------------------------------------------------------
 // CUDA-core route: any head dim that is a multiple of 32 up to 256, any page size, fp32 too.
-// A block takes a tile of up to 16 rows (tokens x heads of a group), four to each warp.
-// Per 32 keys a warp computes four scores per lane (lane = key, q out of shared memory),
-// updates (m, l) by warp reductions, and adds p v with a lane on every 32nd column.  Keys
-// that a row does not see are skipped, so what they hold never reaches it.
+// A block takes a tile of up to 16 rows (tokens x heads of a group), four to each warp.  Its
+// 128 threads bring 32 keys' K and V rows into shared memory as fp32 (while the 32 before them
+// are worked on, where two fit); then per warp a lane takes a key and computes the scores of
+// the warp's four rows (K rows 16 bytes apart modulo the banks: no conflicts), (m, l) move by
+// warp reductions, and for P V a lane takes every 32nd column.  Keys that a row does not see
+// are skipped, so what they hold never reaches it.  Bound by the fp32 FMA pipe for chunks (5
+// shared-memory reads per 16 multiply-adds), by the loads' latency for single tokens.
 // ---------------------------------------------------------------------------
 constexpr int kSimtWarps = 4;
 constexpr int kSimtThreads = 32 * kSimtWarps;
 constexpr int kSimtRows = 4;  // per warp
 constexpr int kSimtTile = kSimtWarps * kSimtRows;
+constexpr int kSimtKeys = 32;  // of a step
+
+template <int DC>
+struct SimtCfg {
+  static constexpr int D = 32 * DC;
+  static constexpr int kKRow = D + 4;  // floats
+  static constexpr int kBuf = kSimtKeys * (kKRow + D);
+  static constexpr int kBufs = DC <= 4 ? 2 : 1;
+  static constexpr int kSmem = 4 * (kBufs * kBuf + kSimtTile * D + kSimtTile * kSimtKeys);
+};
 
 template <typename T>
 struct alignas(16) Vec16 {
@@ -27,10 +40,17 @@ struct alignas(16) Vec16 {
 
 template <typename T, int DC>  // head dim 32 * DC
 __global__ void __launch_bounds__(kSimtThreads) paged_simt_kernel(const Params p) {
-  constexpr int D = 32 * DC;
+  using C = SimtCfg<DC>;
+  constexpr int D = C::D;
   constexpr int VEC = 16 / sizeof(T);
+  constexpr int kVecs = D / VEC;                               // of a row
+  constexpr int kLoads = kSimtKeys * kVecs / kSimtThreads;     // of a thread, K and V each
+  static_assert(kLoads * kSimtThreads == kSimtKeys * kVecs, "whole rows per thread");
+  extern __shared__ float s_mem[];
   __shared__ SchedSmem<kSimtThreads, 1> s_sched;
-  __shared__ float s_q[kSimtTile][D];
+  float* s_kv = s_mem;
+  float* s_q = s_mem + C::kBufs * C::kBuf;  // [row][D]
+  float* s_p = s_q + kSimtTile * D;         // [row][key]
   grid_wait();
   grid_launch_dependents();
   find_work<kSimtThreads, 1>(p, blockIdx.x, s_sched, blockIdx.x == 0);
@@ -39,44 +59,97 @@ __global__ void __launch_bounds__(kSimtThreads) paged_simt_kernel(const Params p
   const Work w = s_sched.found[0];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int subs = p.groups / p.Hkv;  // groups of a KV head
-  const int head0 = w.kvh * p.G + (w.group % subs) * p.group_heads;
+  const int head0 = w.kvh * p.G + (w.group - w.kvh * subs) * p.group_heads;
   const int heads = min(p.group_heads, (w.kvh + 1) * p.G - head0);
   const int tok0 = w.tile * p.tile_tok;  // in the request
   const int n_tok = min(p.tile_tok, w.x.n_tok - tok0);
   const int rows = n_tok * heads;
-  const int pos0 = w.x.seq - w.x.n_tok + tok0;
-  const BlockList list = block_list(p, pos0, pos0 + n_tok - 1);
+  const int pos0 = w.x.seq - w.x.n_tok + tok0, pmax = pos0 + n_tok - 1;
+  const BlockList list = block_list(p, pos0, pmax);
   const int i0 = piece_start(list.n, w.piece, w.pieces);
   const int i1 = piece_start(list.n, w.piece + 1, w.pieces);
   if (w.pieces > 1 && i0 == i1) return;
 
-  for (int i = tid; i < rows * D; i += kSimtThreads) {
-    const int r = i / D, d = i - r * D;
-    const int64_t tok = w.x.tok + tok0 + r / heads;
-    s_q[r][d] = to_f32(static_cast<const T*>(p.q)[tok * p.qs[0] + (head0 + r % heads) * p.qs[1] + d]);
+  const T* kbase = static_cast<const T*>(p.k) + w.kvh * p.ks[1];
+  const T* vbase = static_cast<const T*>(p.v) + w.kvh * p.vs[1];
+  const int* entries = p.table + static_cast<int64_t>(w.r) * p.table_stride;
+  const int block_keys = 1 << p.shift;
+  // steps of 32 keys: the next one that some row of the tile needs, or -1
+  int it_i = i0, it_t = 0;
+  auto next_step = [&]() {
+    for (; it_i < i1; ++it_i, it_t = 0) {
+      const int key0 = list.at(it_i) << p.shift;
+      for (; it_t < block_keys; it_t += kSimtKeys) {
+        const int t = key0 + it_t;
+        if (t > pmax) break;
+        if (t + kSimtKeys <= list.lo_key && t >= p.first) continue;
+        it_t += kSimtKeys;
+        return t;
+      }
+    }
+    return -1;
+  };
+  // This thread's vectors of a step's K and V rows: zeros for keys past the tile's last and for
+  // pages outside the cache.
+  Vec16<T> kreg[kLoads], vreg[kLoads];
+  auto fetch = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int x = tid + i * kSimtThreads, r = x / kVecs, c = x - r * kVecs;
+      const int key = t + r;
+      int pg = -1, col = 0;
+      if (key <= pmax) {
+        col = p.by_page(key);
+        pg = entries[col];
+      }
+      if (pg >= 0 && pg < p.n_pages) {
+        const int64_t off = key - col * p.page;
+        kreg[i] = *reinterpret_cast<const Vec16<T>*>(kbase + pg * p.ks[0] + off * p.ks[2] +
+                                                     c * VEC);
+        vreg[i] = *reinterpret_cast<const Vec16<T>*>(vbase + pg * p.vs[0] + off * p.vs[2] +
+                                                     c * VEC);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) kreg[i].v[e] = vreg[i].v[e] = from_f32<T>(0.f);
+      }
+    }
+  };
+  auto put = [&](float* buf) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int x = tid + i * kSimtThreads, r = x / kVecs, c = x - r * kVecs;
+      float* kd = buf + r * C::kKRow + c * VEC;
+      float* vd = buf + kSimtKeys * C::kKRow + r * D + c * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; e += 4) {
+        *reinterpret_cast<float4*>(kd + e) =
+            make_float4(to_f32(kreg[i].v[e]), to_f32(kreg[i].v[e + 1]),
+                        to_f32(kreg[i].v[e + 2]), to_f32(kreg[i].v[e + 3]));
+        *reinterpret_cast<float4*>(vd + e) =
+            make_float4(to_f32(vreg[i].v[e]), to_f32(vreg[i].v[e + 1]),
+                        to_f32(vreg[i].v[e + 2]), to_f32(vreg[i].v[e + 3]));
+      }
+    }
+  };
+
+  int t = next_step();
+  if (t >= 0) fetch(t);
+  for (int i = tid; i < kSimtTile * D; i += kSimtThreads) {
+    const int r = i / D, e = i - r * D;
+    float x = 0.f;
+    if (r < rows) {
+      const int tk = p.by_head(r);  // (of a partial group the rows are fewer: see below)
+      const int tok_r = heads == p.group_heads ? tk : r / heads;
+      x = to_f32(static_cast<const T*>(p.q)[static_cast<int64_t>(w.x.tok + tok0 + tok_r) * p.qs[0] +
+                                            (head0 + r - tok_r * heads) * p.qs[1] + e]);
+    }
+    s_q[i] = x;
   }
-  __syncthreads();
-  if (warp * kSimtRows >= rows) return;
 
   int pos[kSimtRows];
   float tot_m[kSimtRows], tot_l[kSimtRows], tot_o[kSimtRows][DC];
-#pragma unroll
-  for (int r = 0; r < kSimtRows; ++r) {
-    const int row = warp * kSimtRows + r;
-    // a row that is not there (or whose position is negative) sees nothing
-    pos[r] = row < rows ? max(-1, pos0 + row / heads) : -1;
-    tot_m[r] = -INFINITY;
-    tot_l[r] = 0.f;
-#pragma unroll
-    for (int c = 0; c < DC; ++c) tot_o[r][c] = 0.f;
-  }
-  const int pmax = pos0 + n_tok - 1;
-  const T* kbase = static_cast<const T*>(p.k) + w.kvh * p.ks[1];
-  const T* vbase = static_cast<const T*>(p.v) + w.kvh * p.vs[1];
-
-  for (int i = i0; i < i1; ++i) {
-    const int key0 = list.at(i) * kBlockKeys;
-    float m[kSimtRows], l[kSimtRows], o[kSimtRows][DC];
+  float m[kSimtRows], l[kSimtRows], o[kSimtRows][DC];
+  auto clear = [&]() {
 #pragma unroll
     for (int r = 0; r < kSimtRows; ++r) {
       m[r] = -INFINITY;
@@ -84,84 +157,28 @@ __global__ void __launch_bounds__(kSimtThreads) paged_simt_kernel(const Params p
 #pragma unroll
       for (int c = 0; c < DC; ++c) o[r][c] = 0.f;
     }
-    for (int t = key0; t < key0 + kBlockKeys && t <= pmax; t += 32) {
-      if (t + 31 < list.lo_key && t >= p.first) continue;  // no row sees these
-      const int key = t + lane;
-      unsigned seen[kSimtRows], any = 0;
+  };
+  clear();
 #pragma unroll
-      for (int r = 0; r < kSimtRows; ++r) {
-        const bool see = key <= pos[r] && (key > pos[r] - p.window || key < p.first);
-        seen[r] = __ballot_sync(0xffffffffu, see);
-        any |= seen[r];
-      }
-      if (any == 0) continue;
-      // this lane's key; a page outside the cache reads as zeros
-      int64_t pg = -1;
-      const int col = p.by_page(key);
-      if ((any >> lane) & 1u) pg = p.table[w.r * p.table_stride + col];
-      const bool there = pg >= 0 && pg < p.n_pages;
-      const int64_t off = there ? key - col * p.page : 0;
-      const T* krow = kbase + (there ? pg : 0) * p.ks[0] + off * p.ks[2];
-      int64_t voff = (there ? pg : 0) * p.vs[0] + off * p.vs[2];
-      float s[kSimtRows] = {};
-      if (there) {
-#pragma unroll 4
-        for (int d = 0; d < D; d += VEC) {
-          const Vec16<T> kv = *reinterpret_cast<const Vec16<T>*>(krow + d);
+  for (int r = 0; r < kSimtRows; ++r) {
+    const int row = warp * kSimtRows + r;
+    // a row that is not there (or whose position is negative) sees nothing
+    pos[r] = row < rows ? max(-1, pos0 + row / heads) : -1;
+    tot_m[r] = m[r];
+    tot_l[r] = 0.f;
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float x = to_f32(kv.v[e]);
-#pragma unroll
-            for (int r = 0; r < kSimtRows; ++r) {
-              s[r] = __fmaf_rn(s_q[warp * kSimtRows + r][d + e], x, s[r]);
-            }
-          }
-        }
-      }
-      float pr[kSimtRows];
-#pragma unroll
-      for (int r = 0; r < kSimtRows; ++r) {
-        const bool see = (seen[r] >> lane) & 1u;
-        const float x = see ? __fmul_rn(s[r], p.scale_log2) : -INFINITY;
-        float top = x;
-#pragma unroll
-        for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        const float nm = fmaxf(m[r], top);
-        const float base = nm == -INFINITY ? 0.f : nm;
-        const float f = m[r] == nm ? 1.f : exp2_approx(m[r] - nm);
-        pr[r] = see ? exp2_approx(x - base) : 0.f;
-        float sum = pr[r];
-#pragma unroll
-        for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        m[r] = nm;
-        l[r] = __fmaf_rn(l[r], f, sum);
-#pragma unroll
-        for (int c = 0; c < DC; ++c) o[r][c] = __fmul_rn(o[r][c], f);
-      }
-      const unsigned have = __ballot_sync(0xffffffffu, there);
-      for (unsigned left = any; left != 0; left &= left - 1) {
-        const int j = __ffs(left) - 1;
-        const T* vrow = vbase + __shfl_sync(0xffffffffu, voff, j);
-        float v[DC];
-#pragma unroll
-        for (int c = 0; c < DC; ++c) v[c] = (have >> j) & 1u ? to_f32(vrow[c * 32 + lane]) : 0.f;
-#pragma unroll
-        for (int r = 0; r < kSimtRows; ++r) {
-          const float pj = __shfl_sync(0xffffffffu, pr[r], j);
-          if ((seen[r] >> j) & 1u) {
-#pragma unroll
-            for (int c = 0; c < DC; ++c) o[r][c] = __fmaf_rn(pj, v[c], o[r][c]);
-          }
-        }
-      }
-    }
+    for (int c = 0; c < DC; ++c) tot_o[r][c] = 0.f;
+  }
+  const bool busy = warp * kSimtRows < rows;
+  // The block of the list that `done` is (m, l, o) are complete.
+  auto close_block = [&](int done) {
 #pragma unroll
     for (int r = 0; r < kSimtRows; ++r) {
       const int row = warp * kSimtRows + r;
       if (w.pieces > 1) {
         if (row < rows) {
           const int64_t at = part_slot(p, w.base, w.blocks, tok0 + row / heads,
-                                       head0 + row % heads, i);
+                                       head0 + row % heads, done);
           if (lane == 0) p.part_ml[at] = make_float2(m[r], l[r]);
 #pragma unroll
           for (int c = 0; c < DC; ++c) p.part_o[at * D + c * 32 + lane] = o[r][c];
@@ -174,7 +191,113 @@ __global__ void __launch_bounds__(kSimtThreads) paged_simt_kernel(const Params p
         for (int c = 0; c < DC; ++c) tot_o[r][c] = fold_value(tot_o[r][c], o[r][c], fa, fb);
       }
     }
+    clear();
+  };
+
+  int block = i0;  // being worked on
+  for (int n = 0; t >= 0; ++n) {
+    float* buf = s_kv + (n % C::kBufs) * C::kBuf;
+    if (C::kBufs == 1) __syncthreads();
+    put(buf);
+    __syncthreads();
+    const int now = t;
+    t = next_step();
+    if (t >= 0) fetch(t);
+    if (!busy) continue;
+    while ((list.at(block) << p.shift) + block_keys <= now) close_block(block++);
+    const int key = now + lane;
+    unsigned seen[kSimtRows], any = 0;
+#pragma unroll
+    for (int r = 0; r < kSimtRows; ++r) {
+      const bool see = key <= pos[r] && (key > pos[r] - p.window || key < p.first);
+      seen[r] = __ballot_sync(0xffffffffu, see);
+      any |= seen[r];
+    }
+    if (any == 0) continue;
+    const float* krow = buf + lane * C::kKRow;
+    const float* qrow = s_q + warp * kSimtRows * D;
+    float s[kSimtRows] = {};
+#pragma unroll 8
+    for (int e = 0; e < D; e += 4) {
+      const float4 kv = *reinterpret_cast<const float4*>(krow + e);
+#pragma unroll
+      for (int r = 0; r < kSimtRows; ++r) {
+        const float4 qv = *reinterpret_cast<const float4*>(qrow + r * D + e);
+        s[r] = __fmaf_rn(qv.x, kv.x, s[r]);
+        s[r] = __fmaf_rn(qv.y, kv.y, s[r]);
+        s[r] = __fmaf_rn(qv.z, kv.z, s[r]);
+        s[r] = __fmaf_rn(qv.w, kv.w, s[r]);
+      }
+    }
+    float* prow = s_p + warp * kSimtRows * kSimtKeys;
+#pragma unroll
+    for (int r = 0; r < kSimtRows; ++r) {
+      const bool see = (seen[r] >> lane) & 1u;
+      const float x = see ? __fmul_rn(s[r], p.scale_log2) : -INFINITY;
+      float top = x;
+#pragma unroll
+      for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const float nm = fmaxf(m[r], top);
+      const float base = nm == -INFINITY ? 0.f : nm;
+      const float f = m[r] == nm ? 1.f : exp2_approx(m[r] - nm);
+      const float pr = see ? exp2_approx(x - base) : 0.f;
+      float sum = pr;
+#pragma unroll
+      for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      m[r] = nm;
+      l[r] = __fmaf_rn(l[r], f, sum);
+#pragma unroll
+      for (int c = 0; c < DC; ++c) o[r][c] = __fmul_rn(o[r][c], f);
+      prow[r * kSimtKeys + lane] = pr;
+    }
+    __syncwarp();
+    const float* vbuf = buf + kSimtKeys * C::kKRow + lane;
+    bool every = true;  // rows that are not there have weights of 0 and are not stored
+#pragma unroll
+    for (int r = 0; r < kSimtRows; ++r) {
+      every = every && (seen[r] == 0xffffffffu || warp * kSimtRows + r >= rows);
+    }
+    if (every) {
+#pragma unroll 2
+      for (int j = 0; j < kSimtKeys; j += 4) {
+        float4 pv[kSimtRows];
+#pragma unroll
+        for (int r = 0; r < kSimtRows; ++r) {
+          pv[r] = *reinterpret_cast<const float4*>(prow + r * kSimtKeys + j);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int c = 0; c < DC; ++c) {
+            const float v = vbuf[(j + i) * D + c * 32];
+#pragma unroll
+            for (int r = 0; r < kSimtRows; ++r) {
+              const float pj = i == 0 ? pv[r].x : i == 1 ? pv[r].y : i == 2 ? pv[r].z : pv[r].w;
+              o[r][c] = __fmaf_rn(pj, v, o[r][c]);
+            }
+          }
+        }
+      }
+    } else {
+#pragma unroll 1
+      for (unsigned left = any; left != 0; left &= left - 1) {
+        const int j = __ffs(left) - 1;
+#pragma unroll
+        for (int r = 0; r < kSimtRows; ++r) {
+          if ((seen[r] >> j) & 1u) {
+            const float pj = prow[r * kSimtKeys + j];
+#pragma unroll
+            for (int c = 0; c < DC; ++c) {
+              o[r][c] = __fmaf_rn(pj, vbuf[j * D + c * 32], o[r][c]);
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
   }
+  if (!busy) return;
+  while (block < i1) close_block(block++);
   if (w.pieces > 1) return;
 #pragma unroll
   for (int r = 0; r < kSimtRows; ++r) {
@@ -268,10 +391,11 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
 // kernel here waits for that (grid_wait) before it touches memory.
 template <typename... Args>
 static cudaError_t launch_early(void (*kernel)(Args...), unsigned grid, unsigned block,
-                                cudaStream_t stream, Args... args) {
+                                size_t smem, cudaStream_t stream, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -283,8 +407,14 @@ static cudaError_t launch_early(void (*kernel)(Args...), unsigned grid, unsigned
 
 template <typename T, int DC>
 static int launch_simt(const Params& p, int64_t items, cudaStream_t stream) {
+  constexpr int smem = SimtCfg<DC>::kSmem;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        paged_simt_kernel<T, DC>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(paged_sdpa)");
+  }
   return cuda_status(launch_early(paged_simt_kernel<T, DC>, static_cast<unsigned>(items),
-                                  kSimtThreads, stream, p), "paged_sdpa launch");
+                                  kSimtThreads, smem, stream, p), "paged_sdpa launch");
 }
 template <typename T, int DC>
 static int launch_join(const Params& p, cudaStream_t stream) {
@@ -292,7 +422,7 @@ static int launch_join(const Params& p, cudaStream_t stream) {
   const int64_t want = (rows + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
   const unsigned grid =
       static_cast<unsigned>(std::min<int64_t>(want, 8LL * device_sm_count()));
-  return cuda_status(launch_early(join_kernel<T, DC>, grid, kJoinThreads, stream, p),
+  return cuda_status(launch_early(join_kernel<T, DC>, grid, kJoinThreads, 0, stream, p),
                      "paged_sdpa join launch");
 }
 
@@ -325,7 +455,7 @@ static int64_t info_bytes(int64_t R) { return (16 + 16 * R + 255) / 256 * 256; }
 int64_t paged_sdpa_workspace(int64_t T, int64_t R, int64_t H, int64_t D, int64_t width,
                              int64_t page) {
   const double blocks = static_cast<double>(width) * static_cast<double>(page) /
-                            psdpa::kBlockKeys + 1.0;
+                            (1 << psdpa::kSimtShift) + 1.0;
   const double want = static_cast<double>(T) * static_cast<double>(H) * blocks *
                       static_cast<double>(4 * D + 8);
   const int64_t part = want < static_cast<double>(psdpa::kMaxPartBytes)
@@ -367,7 +497,8 @@ int launch_paged_sdpa(const PagedSdpaArgs& a, cudaStream_t stream) {
   p.G = p.H / p.Hkv;
   p.n_pages = static_cast<int>(a.n_pages);
   p.page = static_cast<int>(a.page);
-  p.max_seq = std::min<int64_t>(a.width * a.page, INT32_MAX - kBlockKeys);
+  p.shift = tc ? kTcShift : kSimtShift;
+  p.max_seq = std::min<int64_t>(a.width * a.page, INT32_MAX - (1 << kTcShift));
   p.group_heads = std::min(p.G, rows);
   p.tile_tok = rows / p.group_heads;
   const int subs = (p.G + rows - 1) / rows;

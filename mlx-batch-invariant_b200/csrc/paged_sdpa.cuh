@@ -4,7 +4,8 @@
 // Arithmetic of a row (query token at position p, one head), the same in every kernel
 // launch and for every split of the work, which is what makes its bits independent of the
 // batch, of how many tokens arrive together and of where its pages lie:
-//   * the keys are taken in blocks of kBlockKeys at fixed positions [512 b, 512 b + 512);
+//   * the keys are taken in blocks of B at fixed positions [B b, B b + B), B = 512 on the
+//     tensor cores and 128 on the CUDA cores;
 //   * a block's partial result (m, l, o) -- running maximum of the scores in units of log 2,
 //     sum of 2^(x - m), and sum of 2^(x - m) v -- starts from nothing in every block;
 //   * partial results are joined in order of the blocks (fold below), in fp32.
@@ -18,7 +19,7 @@
 namespace bi {
 namespace psdpa {
 
-constexpr int kBlockKeys = 512;
+constexpr int kTcShift = 9, kSimtShift = 7;  // log 2 of the keys of a block on either route
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr unsigned kErrReasonRange = 2;
 
@@ -92,6 +93,7 @@ struct Params {
   int T, R, H, Hkv, G;     // G = H / Hkv
   int n_pages, page;
   int64_t max_seq;         // tokens a row of the block table holds
+  int shift;               // log 2 of the keys of a block
   int tile_tok;            // tokens of a tile
   int groups, group_heads; // a KV head's query heads as groups (tiles cover one group)
   Divider by_tile, by_page, by_head, by_group;  // tile_tok, page, group_heads, groups / Hkv
@@ -130,9 +132,9 @@ __device__ __forceinline__ BlockList block_list(const Params& p, int pmin, int p
   b.n = b.n_first = b.first_win = b.lo_key = 0;
   if (pmax < 0) return b;
   if (p.window != INT32_MAX) b.lo_key = max(0, max(pmin, 0) - p.window + 1);
-  const int all = pmax / kBlockKeys + 1;
-  b.first_win = b.lo_key / kBlockKeys;
-  const int firsts = p.first / kBlockKeys + (p.first % kBlockKeys != 0);
+  const int all = (pmax >> p.shift) + 1;
+  b.first_win = b.lo_key >> p.shift;
+  const int firsts = (p.first >> p.shift) + ((p.first & ((1 << p.shift) - 1)) != 0);
   b.n_first = min(firsts, b.first_win);
   b.n = b.n_first + all - b.first_win;
   return b;
@@ -154,10 +156,10 @@ __device__ __forceinline__ int tiles_of(const Params& p, const Request& x) {
 }
 // Most key blocks that any of its tiles lists.
 __device__ __forceinline__ int blocks_of(const Params& p, const Request& x) {
-  const int all = (x.seq + kBlockKeys - 1) / kBlockKeys;
+  const int all = (x.seq + (1 << p.shift) - 1) >> p.shift;
   if (p.window == INT32_MAX) return all;
   const int64_t keys = static_cast<int64_t>(p.window) + min(p.tile_tok, x.n_tok);
-  const int64_t most = p.first / kBlockKeys + keys / kBlockKeys + 3;
+  const int64_t most = (p.first >> p.shift) + (keys >> p.shift) + 3;
   return static_cast<int>(most < all ? most : all);
 }
 

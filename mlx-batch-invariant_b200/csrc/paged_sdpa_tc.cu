@@ -38,6 +38,7 @@ constexpr int kRegsOther = 56;
 constexpr int kTmemCols = 512;        // per item: S (P over its second half) and O, 128 each
 constexpr float kSlack = 8.f;         // log 2 of how far weights may exceed 1
 constexpr int kMaxStages = 12;
+constexpr int kBlockKeys = 1 << kTcShift;
 
 enum : unsigned { kSiteProducer = 1, kSiteMma = 2, kSiteSoftmax = 3, kSiteDrain = 4 };
 

@@ -26,6 +26,7 @@ _i64_2 = _i64 * 2
 
 _lock = threading.Lock()
 _lib = None
+_short = None
 
 
 class LibraryError(RuntimeError):
@@ -38,7 +39,7 @@ class LibraryError(RuntimeError):
                             (": " + detail) if detail else ""))
 
 
-def _bind(lib):
+def _declare(lib):
     lib.bi_gemm.restype = ctypes.c_int
     lib.bi_gemm.argtypes = [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, ctypes.c_int,
                             ctypes.c_float, ctypes.c_float, ctypes.c_int, _vp]
@@ -124,9 +125,25 @@ def lib():
                         "libbi.so is not built (%s); run python mlx-batch-invariant_b200/build.py"
                         % LIB_PATH)
                 handle = ctypes.CDLL(LIB_PATH)
-                _bind(handle)
+                _declare(handle)
                 _lib = handle
     return _lib
+
+
+def short_way():
+    """The _bind module, the short way to the paged-cache operators, set to this libbi.so."""
+    global _short
+    if _short is None:
+        handle = lib()
+        try:
+            from . import _bind as module
+        except ImportError as e:
+            raise RuntimeError("_bind.so is not built (%s); run python "
+                               "mlx-batch-invariant_b200/build.py" % e)
+        module.init(*[ctypes.cast(getattr(handle, name), _vp).value for name in (
+            "bi_paged_plan", "bi_rope_kv_paged", "bi_paged_sdpa", "bi_paged_sdpa_workspace")])
+        _short = module
+    return _short
 
 
 def _status_string(status):

@@ -27,6 +27,7 @@ from . import _lib
 from ._gemm import _check_cuda
 
 MAX_PAGED_HEAD_DIM = 256
+_short = _lib.short_way
 
 
 class PagedPlan(NamedTuple):
@@ -73,6 +74,14 @@ def paged_plan(query_lens, context_lens, block_table, page_size, num_tokens, *, 
     page gets slot -1, and both, like more tokens than ``num_tokens``, are reported by
     ``_lib.device_error()``.
     """
+    compiling = torch.compiler.is_compiling()
+    if not compiling:
+        out = _short().plan(query_lens, context_lens, block_table, page_size, num_tokens,
+                            free_pages, free_head)
+        if out.__class__ is tuple:
+            return PagedPlan._make(out)
+        if out is not None:
+            _lib.check(out, "bi_paged_plan")
     page_size, num_tokens = int(page_size), int(num_tokens)
     if page_size < 1:
         raise ValueError("page_size must be positive, got %d" % page_size)
@@ -88,7 +97,7 @@ def paged_plan(query_lens, context_lens, block_table, page_size, num_tokens, *, 
         _is_vector("free_pages", free_pages, torch.int32)
         _is_vector("free_head", free_head, torch.int32, 1)
     dev = _check_cuda(query_lens, context_lens, block_table, free_pages, free_head)
-    if torch.compiler.is_compiling():
+    if compiling:
         out = torch.ops.mlx_bi.paged_plan(query_lens, context_lens, block_table, page_size,
                                           num_tokens, free_pages, free_head)
         return PagedPlan(*out[:4], out[4] if free_pages is not None else None)
@@ -168,6 +177,13 @@ def rope_kv_paged(qkv, cos, sin, positions, slots, k_cache, v_cache, *, out=None
     tables and slots past the caches write nothing and are reported by
     ``_lib.device_error()``.  The slots of a call must differ.
     """
+    compiling = torch.compiler.is_compiling()
+    if not compiling:
+        q = _short().rope(qkv, cos, sin, positions, slots, k_cache, v_cache, out)
+        if q.__class__ is not int and q is not None:
+            return q
+        if q is not None:
+            _lib.check(q, "bi_rope_kv_paged")
     if qkv.ndim != 2:
         raise ValueError("qkv must be (tokens, (q_heads + 2 kv_heads) * head_dim)")
     _lib.dtype_code(qkv.dtype)
@@ -192,7 +208,7 @@ def rope_kv_paged(qkv, cos, sin, positions, slots, k_cache, v_cache, *, out=None
         raise ValueError("out must be a contiguous (%d, %d, %d) %s tensor" % (T, hq, hd,
                                                                              qkv.dtype))
     dev = _check_cuda(qkv, cos, sin, positions, slots, k_cache, v_cache, out)
-    if torch.compiler.is_compiling():
+    if compiling:
         if out is not None:
             raise NotImplementedError("rope_kv_paged under torch.compile takes no out=")
         return torch.ops.mlx_bi.rope_kv_paged(qkv, cos, sin, positions, slots, k_cache, v_cache)
@@ -234,6 +250,14 @@ def paged_attention(q, k_cache, v_cache, block_table, query_start, seq_lens, *, 
     sees nothing returns zeros.  Lengths are device data; they are clamped to ``q`` and to the
     table, and pages outside the cache read as zeros.
     """
+    compiling = torch.compiler.is_compiling()
+    if not compiling:
+        o = _short().attention(q, k_cache, v_cache, block_table, query_start, seq_lens, scale,
+                               window, first_tokens, sinks, out)
+        if o.__class__ is not int and o is not None:
+            return o
+        if o is not None:
+            _lib.check(o, "bi_paged_sdpa")
     if q.ndim != 3:
         raise ValueError("q must be (tokens, heads, head_dim)")
     code = _lib.dtype_code(q.dtype)
@@ -271,10 +295,10 @@ def paged_attention(q, k_cache, v_cache, block_table, query_start, seq_lens, *, 
                             or (D > 1 and out.stride(2) != 1)):
         raise ValueError("out must be %s %s with a contiguous last dimension"
                          % (tuple(q.shape), q.dtype))
-    if not torch.compiler.is_compiling():
+    if not compiling:
         _check_aligned(k_cache, v_cache)
     dev = _check_cuda(q, k_cache, v_cache, block_table, query_start, seq_lens, sinks, out)
-    if torch.compiler.is_compiling():
+    if compiling:
         if out is not None:
             raise NotImplementedError("paged_attention under torch.compile takes no out=")
         return torch.ops.mlx_bi.paged_attention(q, k_cache, v_cache, block_table, query_start,
