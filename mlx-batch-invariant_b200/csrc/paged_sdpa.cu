@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(kSimtThreads) paged_simt_kernel(const Params p
   float* s_p = s_q + kSimtTile * D;         // [row][key]
   grid_wait();
   grid_launch_dependents();
-  find_work<kSimtThreads, 1>(p, blockIdx.x, s_sched, blockIdx.x == 0);
+  find_work<kSimtThreads, 1>(p, blockIdx.x, 0, s_sched, blockIdx.x == 0);
   __syncthreads();
   if (!s_sched.hit[0]) return;
   const Work w = s_sched.found[0];

@@ -111,10 +111,21 @@ __device__ __forceinline__ int clampi(int64_t v, int64_t lo, int64_t hi) {
   return static_cast<int>(v < lo ? lo : (v > hi ? hi : v));
 }
 
+// n / d: by way of fp32 where that is exact after a correction of one, which is several times
+// shorter than the integer division.
+__device__ __forceinline__ unsigned divide(unsigned n, unsigned d) {
+  if ((n | d) >= (1u << 22)) return n / d;
+  unsigned q = __float2uint_rz(__fdividef(static_cast<float>(n), static_cast<float>(d)));
+  const int rest = static_cast<int>(n - q * d);
+  if (rest < 0) --q;
+  if (rest >= static_cast<int>(d)) ++q;
+  return q;
+}
+
 // Piece `piece` of `pieces` of a list of n blocks: [first, first of the next piece).
 __device__ __forceinline__ int piece_start(int n, int piece, int pieces) {
   if (pieces == 1) return piece == 0 ? 0 : n;
-  const unsigned each = static_cast<unsigned>(n) / static_cast<unsigned>(pieces);
+  const unsigned each = divide(n, pieces);
   return piece * static_cast<int>(each) + min(piece, n - static_cast<int>(each) * pieces);
 }
 
@@ -174,7 +185,7 @@ struct Work {
 template <int NT, int ITEMS>
 struct SchedSmem {
   float f[NT / 32];
-  unsigned a[NT / 32], b[NT / 32];
+  unsigned a[NT / 32], b[NT / 32], c[NT / 32];
   Work found[ITEMS];
   int hit[ITEMS];
 };
@@ -207,6 +218,9 @@ __device__ __forceinline__ void warp_scan(unsigned& a, unsigned& b, int lane) {
 // registers.  Requests whose tiles have few rows (decode), whose partial results are small
 // beside the keys they stand for, are split four times finer (`fine`), so that ragged lengths
 // spread evenly.  The choice changes no bit of the results.
+__device__ __forceinline__ bool few_rows(const Params& p, const Request& x) {
+  return min(x.n_tok, p.tile_tok) * p.group_heads <= p.fine_rows;
+}
 struct Spans {
   unsigned span, fine;
 };
@@ -221,8 +235,8 @@ __device__ __forceinline__ float load_of(const Params& p, const Request& x) {
 }
 __device__ __forceinline__ unsigned pieces_of(const Params& p, const Request& x, const Spans& s,
                                               int tiles, int blocks, unsigned& slots) {
-  const unsigned most = min(x.n_tok, p.tile_tok) * p.group_heads <= p.fine_rows ? s.fine : s.span;
-  const unsigned pieces = tiles == 0 ? 0 : max(1u, (blocks + most - 1) / most);
+  const unsigned most = few_rows(p, x) ? s.fine : s.span;
+  const unsigned pieces = tiles == 0 ? 0 : max(1u, divide(blocks + most - 1, most));
   const float want = static_cast<float>(x.n_tok) * static_cast<float>(p.H) *
                      static_cast<float>(blocks);
   slots = pieces <= 1 ? 0u : want >= static_cast<float>(kMuch) ? kMuch
@@ -247,58 +261,82 @@ __device__ __forceinline__ void take_items(const Params& p, int item, SchedSmem<
     w.blocks = blocks;
     w.base = base;
     w.x = x;
-    w.group = in / per_group;
-    const unsigned rest = in - w.group * per_group;
-    w.tile = tiles - 1 - static_cast<int>(rest / pieces);
-    w.piece = rest % pieces;
+    w.group = divide(in, per_group);
+    const unsigned rest = in - w.group * per_group, q = divide(rest, pieces);
+    w.tile = tiles - 1 - static_cast<int>(q);
+    w.piece = rest - q * pieces;
     w.kvh = p.by_group(w.group);
     s.found[k] = w;
     s.hit[k] = 1;
   }
 }
 
-// Finds items item .. item + ITEMS - 1 of the call, with all threads of the block (NT); the
-// answer is in `s` after the block's next barrier.  Items go request by request, in a request
-// group of heads by group, tile by tile from the last (in causal attention the longest) to the
-// first, piece by piece of a tile's keys.  Up to 64 requests one warp does it in registers;
-// beyond, the block scans them 32 a warp at a time.  The block that `publish`es leaves the
-// split of every request for the join.
+// Finds the work of block `blk` of the call, with all threads of the block (NT); the answer is
+// in `s` after the block's next barrier (after __syncwarp for warp 0, if there are at most 64
+// requests).  Block b takes items ITEMS b ... of the call, or, as long as there are no more
+// items than `spread`, item b alone.  Items go request by request -- first the requests whose
+// tiles have many rows, whose items are the long ones -- in a request group of heads by group,
+// tile by tile from the last (in causal attention the longest) to the first, piece by piece of
+// a tile's keys.  Up to 64 requests one warp does it in registers; beyond, the block scans
+// them 32 a warp at a time.  The block that `publish`es leaves the split of every request for
+// the join.
 template <int NT, int ITEMS>
-__device__ __forceinline__ void find_work(const Params& p, int item, SchedSmem<NT, ITEMS>& s,
-                                          bool publish) {
+__device__ __forceinline__ void find_work(const Params& p, int blk, int spread,
+                                          SchedSmem<NT, ITEMS>& s, bool publish) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (p.R <= 64) {
     if (warp != 0) return;
     if (lane < ITEMS) s.hit[lane] = 0;
     __syncwarp();
+    const int halves = p.R > 32 ? 2 : 1;
     Request x[2];
+    int tiles[2], blocks[2];
     float load = 0.f;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = lane + 32 * h;
       x[h] = r < p.R ? request(p, r) : Request{0, 0, 0};
-      load += load_of(p, x[h]);
+      tiles[h] = tiles_of(p, x[h]);
+      blocks[h] = blocks_of(p, x[h]);
+      load += static_cast<float>(tiles[h]) * static_cast<float>(blocks[h]);
     }
     const Spans sp = spans_of(p, warp_sum(load));
-    unsigned items0 = 0, slots0 = 0, split = 0;
+    unsigned pieces[2] = {0, 0}, base[2], at[2], items[2];
+    unsigned slots0 = 0, many0 = 0, few0 = 0, split = 0;
+    bool few[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = lane + 32 * h, tiles = tiles_of(p, x[h]), blocks = blocks_of(p, x[h]);
+      at[h] = base[h] = items[h] = 0;
+      few[h] = few_rows(p, x[h]);
+      if (h >= halves) continue;
       unsigned slots;
-      unsigned pieces = pieces_of(p, x[h], sp, tiles, blocks, slots);
+      pieces[h] = pieces_of(p, x[h], sp, tiles[h], blocks[h], slots);
       unsigned none = 0, ends = slots;
-      warp_scan(none, ends, lane);
-      const unsigned base = add_sat(slots0, ends) - slots;  // (exact below kMuch)
-      if (pieces > 1 && add_sat(slots0, ends) > p.slots) pieces = 1;
-      const unsigned items = tiles * pieces * p.groups;
-      unsigned at = items;
-      warp_scan(at, none, lane);
+      if (__any_sync(0xffffffffu, slots != 0)) warp_scan(none, ends, lane);
+      base[h] = add_sat(slots0, ends) - slots;  // (exact below kMuch)
+      if (pieces[h] > 1 && add_sat(slots0, ends) > p.slots) pieces[h] = 1;  // no room for them
       slots0 = add_sat(slots0, __shfl_sync(0xffffffffu, ends, 31));
-      take_items(p, item, s, r, x[h], tiles, blocks, pieces, base, items0 + at - items, items);
-      items0 += __shfl_sync(0xffffffffu, at, 31);
-      if (publish && r < p.R) p.info[r] = make_int4(pieces, blocks, base, 0);
-      split |= pieces > 1;
+      items[h] = tiles[h] * pieces[h] * p.groups;
+      unsigned m = few[h] ? 0 : items[h], f = items[h] - m;
+      warp_scan(m, f, lane);
+      at[h] = few[h] ? few0 + f - items[h] : many0 + m - items[h];
+      many0 += __shfl_sync(0xffffffffu, m, 31);
+      few0 += __shfl_sync(0xffffffffu, f, 31);
+      split |= pieces[h] > 1;
     }
+    const int per = many0 + few0 <= static_cast<unsigned>(spread) ? 1 : ITEMS;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = lane + 32 * h;
+      if (few[h]) at[h] += many0;
+      if (items[h] != 0) {
+        take_items(p, blk * per, s, r, x[h], tiles[h], blocks[h], pieces[h], base[h], at[h],
+                   items[h]);
+      }
+      if (publish && r < p.R) p.info[r] = make_int4(pieces[h], blocks[h], base[h], 0);
+    }
+    __syncwarp();
+    if (lane >= per && lane < ITEMS) s.hit[lane] = 0;
     if (publish) {
       split = __any_sync(0xffffffffu, split);
       if (lane == 0) *p.any_split = split;
@@ -315,41 +353,61 @@ __device__ __forceinline__ void find_work(const Params& p, int item, SchedSmem<N
 #pragma unroll
   for (int w = 0; w < NT / 32; ++w) load += s.f[w];
   const Spans sp = spans_of(p, load);
-  unsigned items0 = 0, slots0 = 0, split = 0;
-  for (int r0 = 0; r0 < p.R; r0 += NT) {
-    const int r = r0 + tid;
-    const Request x = r < p.R ? request(p, r) : Request{0, 0, 0};
-    const int tiles = tiles_of(p, x), blocks = blocks_of(p, x);
-    unsigned slots, none = 0;
-    unsigned pieces = pieces_of(p, x, sp, tiles, blocks, slots);
-    unsigned ends = slots;
-    warp_scan(none, ends, lane);
-    if (lane == 31) s.b[warp] = ends;
-    __syncthreads();
-    unsigned total = 0;
+  // pass 0 counts the items, pass 1 places them
+  unsigned split = 0, many_all = 0;
+  int per = ITEMS;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    unsigned many0 = 0, few0 = 0, slots0 = 0;
+#pragma unroll 1
+    for (int r0 = 0; r0 < p.R; r0 += NT) {
+      const int r = r0 + tid;
+      const Request x = r < p.R ? request(p, r) : Request{0, 0, 0};
+      const int tiles = tiles_of(p, x), blocks = blocks_of(p, x);
+      const bool few = few_rows(p, x);
+      unsigned slots, none = 0;
+      unsigned pieces = pieces_of(p, x, sp, tiles, blocks, slots);
+      unsigned ends = slots;
+      warp_scan(none, ends, lane);
+      if (lane == 31) s.b[warp] = ends;
+      __syncthreads();
+      unsigned total = 0;
 #pragma unroll
-    for (int w = 0; w < NT / 32; ++w) {
-      if (w == warp) ends = add_sat(ends, add_sat(slots0, total));
-      total = add_sat(total, s.b[w]);
-    }
-    slots0 = add_sat(slots0, total);
-    if (pieces > 1 && ends > p.slots) pieces = 1;  // no room for its partial results
-    const unsigned items = tiles * pieces * p.groups;
-    unsigned at = items;
-    warp_scan(at, none, lane);
-    if (lane == 31) s.a[warp] = at;
-    __syncthreads();
-    at += items0 - items;
+      for (int w = 0; w < NT / 32; ++w) {
+        if (w == warp) ends = add_sat(ends, add_sat(slots0, total));
+        total = add_sat(total, s.b[w]);
+      }
+      slots0 = add_sat(slots0, total);
+      if (pieces > 1 && ends > p.slots) pieces = 1;  // no room for its partial results
+      const unsigned items = tiles * pieces * p.groups;
+      unsigned m = few ? 0 : items, f = items - m;
+      warp_scan(m, f, lane);
+      if (lane == 31) {
+        s.a[warp] = m;
+        s.c[warp] = f;
+      }
+      __syncthreads();
+      unsigned at = few ? few0 + f - items : many0 + m - items;
 #pragma unroll
-    for (int w = 0; w < NT / 32; ++w) {
-      if (w < warp) at += s.a[w];
-      items0 += s.a[w];
+      for (int w = 0; w < NT / 32; ++w) {
+        if (w < warp) at += few ? s.c[w] : s.a[w];
+        many0 += s.a[w];
+        few0 += s.c[w];
+      }
+      if (pass == 1) {
+        if (few) at += many_all;
+        if (items != 0) {
+          take_items(p, blk * per, s, r, x, tiles, blocks, pieces, ends - slots, at, items);
+        }
+        if (publish && r < p.R) p.info[r] = make_int4(pieces, blocks, ends - slots, 0);
+        split |= pieces > 1;
+      }
     }
-    take_items(p, item, s, r, x, tiles, blocks, pieces, ends - slots, at, items);
-    if (publish && r < p.R) p.info[r] = make_int4(pieces, blocks, ends - slots, 0);
-    split |= pieces > 1;
-    if (!publish && items0 >= static_cast<unsigned>(item + ITEMS)) break;  // (uniform)
+    many_all = many0;
+    per = many0 + few0 <= static_cast<unsigned>(spread) ? 1 : ITEMS;
   }
+  __syncthreads();
+  if (tid >= per && tid < ITEMS) s.hit[tid] = 0;
   if (publish) {
     split = __syncthreads_or(split);
     if (tid == 0) *p.any_split = split;

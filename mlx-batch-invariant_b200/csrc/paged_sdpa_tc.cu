@@ -25,6 +25,8 @@
 // row sees only in part the V rows are looked over in shared memory: what no row of the block
 // sees is zeroed, and a non-finite value that some rows see is taken out of the product and
 // added to those rows' results by hand.
+#include <algorithm>
+
 #include "paged_sdpa.cuh"
 
 namespace bi {
@@ -252,10 +254,10 @@ __device__ __forceinline__ unsigned steps_of(const Params& p, const Item& it, in
   return set;
 }
 
-// Describes item k of the block; a whole warp.
-__device__ __forceinline__ void make_item(const Params& p, const SchedSmem<kThreads, 2>& s, int k,
-                                          bool shared, Item& out) {
-  const int lane = threadIdx.x & 31;
+// Describes both items of the block, 16 lanes of a warp each.
+__device__ __forceinline__ void make_items(const Params& p, const SchedSmem<kThreads, 2>& s,
+                                           bool shared, Item (&out)[2]) {
+  const int lane = threadIdx.x & 15, k = (threadIdx.x & 31) >> 4;
   Item it;
   it.pieces = 0;
   it.r = it.kvh = it.tok = it.base = it.blocks = 0;
@@ -285,11 +287,14 @@ __device__ __forceinline__ void make_item(const Params& p, const SchedSmem<kThre
     it.list = block_list(p, it.list_pos0, it.list_pmax);
     it.i0 = piece_start(it.list.n, w.piece, w.pieces);
     it.i1 = piece_start(it.list.n, w.piece + 1, w.pieces);
-    unsigned n = 0;
-    for (int i = it.i0 + lane; i < it.i1; i += 32) n += __popc(steps_of(p, it, it.list.at(i)));
-    it.steps = static_cast<int>(__reduce_add_sync(0xffffffffu, n));
+    for (int i = it.i0 + lane; i < it.i1; i += 16) {
+      it.steps += __popc(steps_of(p, it, it.list.at(i)));
+    }
   }
-  if (lane == 0) out = it;
+  __syncwarp();
+#pragma unroll
+  for (int d = 8; d > 0; d /= 2) it.steps += __shfl_xor_sync(0xffffffffu, it.steps, d);
+  if (lane == 0) out[k] = it;
 }
 
 // Walks an item's steps.
@@ -327,6 +332,7 @@ struct Shared {
       o_full[2], mma_done;
   uint32_t tmem;
   int abort_flag;
+  int shared;             // the items share K and V
   Item item[2];
   int keep_o[2];          // the softmax warps put values into O: accumulate on them
   unsigned bad[2][2][4];  // keys of a step with a non-finite value that some row sees
@@ -337,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     paged_tc_kernel(const __grid_constant__ CUtensorMap map_q,
                     const __grid_constant__ CUtensorMap map_q1,
                     const __grid_constant__ CUtensorMap map_k,
-                    const __grid_constant__ CUtensorMap map_v, const Params p) {
+                    const __grid_constant__ CUtensorMap map_v, const Params p, int n_sm) {
   using C = Cfg<D>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared sh;
@@ -354,17 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
   }
-  grid_wait();
-  grid_launch_dependents();
-  find_work<kThreads, 2>(p, 2 * blockIdx.x, sh.sched, blockIdx.x == 0);
-  __syncthreads();
-  if (!sh.sched.hit[0]) return;
-  // two tiles of one request and group, their keys not split: they share K and V
-  const bool shared = sh.sched.hit[1] && sh.sched.found[0].r == sh.sched.found[1].r &&
-                      sh.sched.found[0].group == sh.sched.found[1].group &&
-                      sh.sched.found[0].pieces == 1;
-
-  if (tid == 0) {
+  if (warp == 10 && lane == 0) {
     for (int k = 0; k < 2; ++k) {
       mbar_init(&sh.q_full[k], 1);
       mbar_init(&sh.s_full[k], 1);
@@ -375,17 +371,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&sh.full[s], 1);
-      mbar_init(&sh.empty[s], shared ? 2 : 1);
+      mbar_init(&sh.empty[s], 1);
     }
     mbar_init(&sh.mma_done, 1);
     sh.abort_flag = 0;
     fence_barrier_init();
   }
+  grid_wait();
+  grid_launch_dependents();
+  find_work<kThreads, 2>(p, blockIdx.x, n_sm, sh.sched, blockIdx.x == 0);
+  if (p.R > 64) __syncthreads();
+  if (warp == 0) {
+    __syncwarp();
+    // two tiles of one request and group, their keys not split: they share K and V
+    const bool both = sh.sched.hit[0] && sh.sched.hit[1] &&
+                      sh.sched.found[0].r == sh.sched.found[1].r &&
+                      sh.sched.found[0].group == sh.sched.found[1].group &&
+                      sh.sched.found[0].pieces == 1;
+    make_items(p, sh.sched, both, sh.item);
+    if (lane == 0) sh.shared = both;
+  }
+  __syncthreads();
+  if (sh.item[0].pieces == 0) return;
+  const bool shared = sh.shared;
   if (warp == 9) {
     tmem_alloc(&sh.tmem, kTmemCols);
     tmem_relinquish();
   }
-  if (warp == 4 || warp == 7) make_item(p, sh.sched, warp == 7, shared, sh.item[warp == 7]);
   __syncwarp();
   tc_fence_before();
   __syncthreads();
@@ -555,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int i = 0; i < 4; ++i) {
                 umma_f16_ts(d + 128, d + 64 + i * 8, vd + i * (2048 >> 4), idesc_o, true);
               }
-              umma_commit(&sh.empty[stage]);
+              if (!both || k == 1) umma_commit(&sh.empty[stage]);
               if (j + 1 == steps) umma_commit(&sh.o_full[k]);
             }
             __syncwarp();
@@ -572,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint64_t off = ((i / 4) * (kTile * 128) + (i % 4) * 32) >> 4;
                 umma_f16(tm + 256 * k, qd + off, kd + off, idesc_s, i != 0 ? 1u : 0u);
               }
-              umma_commit(&sh.empty[ks]);
+              if (!both || k == 1) umma_commit(&sh.empty[ks]);
               umma_commit(&sh.s_full[k]);
             }
             __syncwarp();
@@ -693,13 +705,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (warp_live) {
         if (__builtin_expect(!whole, 0)) {  // keys that the row does not see: a score of -inf
 #pragma unroll 1
-          for (int b = 0; b < 4; ++b) {
-            const uint32_t word = b == 0 ? vis[0] : b == 1 ? vis[1] : b == 2 ? vis[2] : vis[3];
-            tmem_ld_32x32b_x32(tS + 32 * b, sa);
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t wa = h == 0 ? vis[0] : vis[2], wb = h == 0 ? vis[1] : vis[3];
+            tmem_ld_32x32b_x32(tS + 64 * h, sa);
+            tmem_ld_32x32b_x32(tS + 64 * h + 32, sb);
             tmem_ld_wait(sa);
+            tmem_ld_wait(sb);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) sa[j] = (word >> j) & 1u ? sa[j] : 0xff800000u;
-            tmem_st_x32(tS + 32 * b, sa);
+            for (int j = 0; j < 32; ++j) {
+              sa[j] = (wa >> j) & 1u ? sa[j] : 0xff800000u;
+              sb[j] = (wb >> j) & 1u ? sb[j] : 0xff800000u;
+            }
+            tmem_st_x32(tS + 64 * h, sa);
+            tmem_st_x32(tS + 64 * h + 32, sb);
           }
           tmem_st_wait();
         }
@@ -762,33 +780,52 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint8_t* vrow = s_ring + stage * C::kTileBytes + row * 128;
         const int key = t0 + row;
         const bool seen = key <= item.list_pmax && (key >= item.list.lo_key || key < p.first);
-        constexpr uint32_t em = exp_mask<T>();
-        constexpr int kChunks = C::kHalves * 8;
+        // seen by every row: nothing to do.  By some: look for non-finite values.  By none: zeros.
+        const bool by_all = key <= item.list_pos0 &&
+                            (p.window == INT32_MAX || key > item.list_pmax - p.window ||
+                             key < p.first);
+        constexpr uint32_t em = exp_mask<T>() * 0x10001u;           // both values' exponents
+        constexpr uint32_t one = (exp_mask<T>() & -exp_mask<T>()) * 0x10001u;
+        constexpr int kChunks = C::kHalves * 8 / 2;
         bool found = false;
-        const int c0 = shared ? k * (kChunks / 2) : 0;
-        const int c1 = shared ? c0 + kChunks / 2 : kChunks;
 #pragma unroll 1
-        for (int c = c0; c < c1; ++c) {
-          uint4* at = reinterpret_cast<uint4*>(vrow + (c >> 3) * (kTile * 128) +
-                                               (((c ^ row) & 7) << 4));
-          uint4 x = *at;
-          uint32_t* xw = reinterpret_cast<uint32_t*>(&x);
-          bool hit = false;
+        for (int part = shared ? k : 0; part < (shared ? k + 1 : 2); ++part) {
+          // 16-byte chunk c of a row sits at c ^ (row & 7) of its 128 bytes
+          auto chunk = [&](int c) {
+            const int at = part * kChunks + c;
+            return reinterpret_cast<uint4*>(vrow + (at >> 3) * (kTile * 128) +
+                                            (((at ^ row) & 7) << 4));
+          };
+          if (by_all) continue;
+          uint32_t hit = seen ? 0u : 0x8000u;
+          if (seen) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if ((xw[e] & em) == em) {
-              xw[e] &= 0xffff0000u;
-              hit = true;
-            }
-            if (((xw[e] >> 16) & em) == em) {
-              xw[e] &= 0xffffu;
-              hit = true;
+            for (int c = 0; c < kChunks; ++c) {
+              const uint4 x = *chunk(c);
+              // an exponent of all ones carries into the sign's place
+              hit |= ((x.x & em) + one) | ((x.y & em) + one) | ((x.z & em) + one) |
+                     ((x.w & em) + one);
             }
           }
-          if (hit) *at = x;
-          found |= hit;
+          if ((hit & 0x80008000u) == 0) continue;
+          found |= seen;
+#pragma unroll 1
+          for (int c = 0; c < kChunks; ++c) {
+            uint4* at = chunk(c);
+            uint4 x = seen ? *at : make_uint4(0u, 0u, 0u, 0u);
+            if (seen) {
+              uint32_t* xw = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t top = ((xw[e] & em) + one) & 0x80008000u;
+                if (top & 0x8000u) xw[e] &= 0xffff0000u;
+                if (top & 0x80000000u) xw[e] &= 0xffffu;
+              }
+            }
+            *at = x;
+          }
         }
-        const unsigned flags = __ballot_sync(0xffffffffu, found && seen);
+        const unsigned flags = __ballot_sync(0xffffffffu, found);
         const int buf = scans++ & 1;
         if (lane == 0) sh.bad[buf][k][warp & 3] = flags;
         fence_proxy_async_smem();  // the zeros, to the product's reads
@@ -933,7 +970,10 @@ static int launch(const PagedSdpaArgs& a, const Params& p, int64_t items, cudaSt
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(paged_sdpa)");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((items + 1) / 2));
+  // two items a block, or one while there are no more items than SMs
+  const int n_sm = device_sm_count();
+  cfg.gridDim = dim3(static_cast<unsigned>(std::max<int64_t>((items + 1) / 2,
+                                                             std::min<int64_t>(items, n_sm))));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = stream;
@@ -942,7 +982,7 @@ static int launch(const PagedSdpaArgs& a, const Params& p, int64_t items, cudaSt
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, paged_tc_kernel<T, D>, mq, mq1, mk, mv, p),
+  return cuda_status(cudaLaunchKernelEx(&cfg, paged_tc_kernel<T, D>, mq, mq1, mk, mv, p, n_sm),
                      "paged_sdpa tensor-core launch");
 }
 
