@@ -47,16 +47,23 @@ __global__ void __launch_bounds__(kSimtThreads) paged_simt_kernel(const Params p
   constexpr int kLoads = kSimtKeys * kVecs / kSimtThreads;     // of a thread, K and V each
   static_assert(kLoads * kSimtThreads == kSimtKeys * kVecs, "whole rows per thread");
   extern __shared__ float s_mem[];
-  __shared__ SchedSmem<kSimtThreads, 1> s_sched;
+  __shared__ Work s_work;
+  __shared__ int s_there;
   float* s_kv = s_mem;
   float* s_q = s_mem + C::kBufs * C::kBuf;  // [row][D]
   float* s_p = s_q + kSimtTile * D;         // [row][key]
   grid_wait();
   grid_launch_dependents();
-  find_work<kSimtThreads, 1>(p, blockIdx.x, 0, s_sched, blockIdx.x == 0);
+  if (threadIdx.x < 32) {
+    Finder finder;
+    finder.begin(p, blockIdx.x == 0);
+    const bool there = blockIdx.x < finder.total;
+    if (there) finder.find(p, blockIdx.x, &s_work);
+    if (threadIdx.x == 0) s_there = there;
+  }
   __syncthreads();
-  if (!s_sched.hit[0]) return;
-  const Work w = s_sched.found[0];
+  if (!s_there) return;
+  const Work w = s_work;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int subs = p.groups / p.Hkv;  // groups of a KV head
   const int head0 = w.kvh * p.G + (w.group - w.kvh * subs) * p.group_heads;
@@ -314,6 +321,63 @@ __global__ void __launch_bounds__(kSimtThreads) paged_simt_kernel(const Params p
 }
 
 // ---------------------------------------------------------------------------
+// The items of calls with more requests than a warp keeps in registers: one block, ahead of the
+// main kernel, leaves every request's split and the running numbers of items.
+// ---------------------------------------------------------------------------
+constexpr int kScheduleThreads = 1024;
+
+__global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const Params p) {
+  constexpr int kWarps = kScheduleThreads / 32;
+  __shared__ float s_load[kWarps];
+  __shared__ unsigned s_slots[kWarps], s_many[kWarps], s_few[kWarps];
+  grid_wait();
+  grid_launch_dependents();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  float load = 0.f;
+  for (int r = tid; r < p.R; r += kScheduleThreads) load += load_of(share_of(p, r));
+  load = warp_sum(load);
+  if (lane == 0) s_load[warp] = load;
+  __syncthreads();
+  const Spans sp = spans_of(p, warp_sum(s_load[lane]));
+  unsigned slots0 = 0, many0 = 0, few0 = 0;
+  int split = 0;
+  for (int r0 = 0; r0 < p.R; r0 += kScheduleThreads) {
+    const int r = r0 + tid;
+    Share s = share_of(p, r);
+    split_share(p, sp, s);
+    const unsigned in_warp = warp_scan(s.slots);
+    if (lane == 31) s_slots[warp] = in_warp;
+    __syncthreads();
+    const unsigned slots = warp_scan(s_slots[lane]);  // up to warp `lane`'s end
+    unsigned before = __shfl_sync(0xffffffffu, slots, max(warp - 1, 0));
+    const unsigned end = add_sat(add_sat(slots0, warp > 0 ? before : 0u), in_warp);
+    slots0 = add_sat(slots0, __shfl_sync(0xffffffffu, slots, 31));
+    count_items(p, end, s);
+    const unsigned m_in = warp_scan(s.few ? 0 : s.items), f_in = warp_scan(s.few ? s.items : 0);
+    if (lane == 31) {
+      s_many[warp] = m_in;
+      s_few[warp] = f_in;
+    }
+    __syncthreads();
+    const unsigned m = warp_scan(s_many[lane]), f = warp_scan(s_few[lane]);
+    before = __shfl_sync(0xffffffffu, m, max(warp - 1, 0));
+    const unsigned m_end = many0 + (warp > 0 ? before : 0u) + m_in;
+    before = __shfl_sync(0xffffffffu, f, max(warp - 1, 0));
+    const unsigned f_end = few0 + (warp > 0 ? before : 0u) + f_in;
+    many0 += __shfl_sync(0xffffffffu, m, 31);
+    few0 += __shfl_sync(0xffffffffu, f, 31);
+    if (r < p.R) {
+      p.info[r] = make_int4(s.pieces, s.blocks, end - s.slots, 0);
+      p.ends[r] = make_int2(m_end, f_end);
+    }
+    split |= s.pieces > 1;
+    __syncthreads();
+  }
+  split = __syncthreads_or(split);
+  if (tid == 0) *p.head = make_int4(many0, few0, split, 0);
+}
+
+// ---------------------------------------------------------------------------
 // Join of the partial results of split requests: a warp takes one row (token, head) and
 // folds its blocks' partial results in order, with the operations of the unsplit kernels.
 // Launched behind every call (the split is decided on the device); where nothing was split
@@ -326,7 +390,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
   constexpr int D = 32 * DC;
   constexpr int kAhead = 8;  // partial results in flight
   grid_wait();
-  if (*p.any_split == 0) return;
+  if (p.head->z == 0) return;
   const int lane = threadIdx.x & 31;
   const int64_t n_rows = static_cast<int64_t>(p.T) * p.H;
   const int64_t warps = static_cast<int64_t>(gridDim.x) * (kJoinThreads / 32);
@@ -446,7 +510,7 @@ static int dispatch(const Params& p, int dtype, int64_t D, int64_t items, bool j
 
 constexpr int64_t kMaxPartBytes = 256LL << 20;
 
-static int64_t info_bytes(int64_t R) { return (16 + 16 * R + 255) / 256 * 256; }
+static int64_t info_bytes(int64_t R) { return (16 + 24 * R + 255) / 256 * 256; }
 
 }  // namespace psdpa
 
@@ -507,11 +571,11 @@ int launch_paged_sdpa(const PagedSdpaArgs& a, cudaStream_t stream) {
   p.by_page = divider(a.page);
   p.by_head = divider(p.group_heads);
   p.by_group = divider(subs);
-  p.target = (tc ? 2 : 8) * device_sm_count();
-  p.fine_rows = 16;
+  p.target = 2 * device_sm_count();
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
-  p.any_split = reinterpret_cast<int*>(ws);
+  p.head = reinterpret_cast<int4*>(ws);
   p.info = reinterpret_cast<int4*>(ws + 16);
+  p.ends = reinterpret_cast<int2*>(ws + 16 + 16 * a.R);
   const int64_t left = a.workspace_bytes - info_bytes(a.R);
   p.slots = left <= 256 ? 0u : static_cast<unsigned>(
       std::min<int64_t>((left - 256) / (4 * a.D + 8), kMuch - 1));
@@ -520,9 +584,17 @@ int launch_paged_sdpa(const PagedSdpaArgs& a, cudaStream_t stream) {
 
   // tiles of all requests: at most one ragged tile each
   const int64_t tiles = a.T / p.tile_tok + std::min(a.R, a.T);
-  // (the spans are rounded in fp32: a little above 4 target pieces)
-  const int64_t items = tiles * p.groups + 4LL * p.target + 64;
+  p.fine_rows = 16;
+  // few tiles: one piece for every place is enough; many: finer, to even out ragged lengths
+  p.finer = tiles * p.groups >= p.target ? 4 : 1;
+  // (the spans are rounded in fp32: a little above finer x target pieces)
+  const int64_t items = tiles * p.groups + static_cast<int64_t>(p.finer) * p.target + 64;
   if (items > INT32_MAX) return set_error(BI_ERR_UNSUPPORTED, "too many query tiles");
+  if (a.R > kFewRequests) {
+    const int st = cuda_status(launch_early(schedule_kernel, 1u, kScheduleThreads, 0, stream, p),
+                               "paged_sdpa schedule launch");
+    if (st) return st;
+  }
   const int st = tc ? launch_paged_tc(a, p, items, stream)
                     : dispatch(p, a.dtype, a.D, items, false, stream);
   if (st) return st;

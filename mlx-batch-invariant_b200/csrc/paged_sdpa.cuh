@@ -98,10 +98,12 @@ struct Params {
   int groups, group_heads; // a KV head's query heads as groups (tiles cover one group)
   Divider by_tile, by_page, by_head, by_group;  // tile_tok, page, group_heads, groups / Hkv
   int target;              // work items to aim for when a request's keys are split
-  int fine_rows;           // tiles of at most so many rows are cheap to split
+  int fine_rows;           // tiles of at most so many rows are cheap to split ...
+  int finer;               // ... so many times finer
   // partial results of split requests
+  int4* head;              // {items of many rows, of few rows, whether a request is split, -}
   int4* info;              // per request {pieces, blocks a row has, first slot, -}
-  int* any_split;
+  int2* ends;              // per request {items of many rows up to its own, of few rows}
   float2* part_ml;         // (slot,) (m, l)
   float* part_o;           // (slot, D)
   unsigned slots;
@@ -181,15 +183,6 @@ struct Work {
   Request x;
 };
 
-// The work of a block: ITEMS consecutive items of the call.
-template <int NT, int ITEMS>
-struct SchedSmem {
-  float f[NT / 32];
-  unsigned a[NT / 32], b[NT / 32], c[NT / 32];
-  Work found[ITEMS];
-  int hit[ITEMS];
-};
-
 constexpr unsigned kMuch = 1u << 30;  // sums of slots stop here (the workspace holds fewer)
 __device__ __forceinline__ unsigned add_sat(unsigned a, unsigned b) { return min(a + b, kMuch); }
 
@@ -198,221 +191,179 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int d = 16; d > 0; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
   return v;
 }
-// Inclusive scans of item counts and (saturating) slot counts over a warp.
-__device__ __forceinline__ void warp_scan(unsigned& a, unsigned& b, int lane) {
+// Inclusive scan over a warp (sums above kMuch stay there).
+__device__ __forceinline__ unsigned warp_scan(unsigned a) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
-    const unsigned x = __shfl_up_sync(0xffffffffu, a, d), y = __shfl_up_sync(0xffffffffu, b, d);
-    if (lane >= d) {
-      a += x;
-      b = add_sat(b, y);
-    }
+    const unsigned x = __shfl_up_sync(0xffffffffu, a, d);
+    if (lane >= d) a = add_sat(a, x);
   }
+  return a;
 }
 
-// Into how many pieces the keys of a request's tiles are split, and the slots that its partial
-// results then take.
+// The items of a call: request by request -- first the requests whose tiles have many rows,
+// whose items are the long ones -- in a request group of heads by group, tile by tile from the
+// last (in causal attention the longest) to the first, piece by piece of a tile's keys.
 //
-// A request's keys are split only where that shortens the call: a tile whose blocks are at
-// most the average load (`span`) is computed in one go, which then keeps the fold in
+// A request's keys are split into pieces only where that shortens the call: a tile whose blocks
+// are at most the average load (`span`) is computed in one go, which then keeps the fold in
 // registers.  Requests whose tiles have few rows (decode), whose partial results are small
-// beside the keys they stand for, are split four times finer (`fine`), so that ragged lengths
-// spread evenly.  The choice changes no bit of the results.
-__device__ __forceinline__ bool few_rows(const Params& p, const Request& x) {
-  return min(x.n_tok, p.tile_tok) * p.group_heads <= p.fine_rows;
-}
+// beside the keys they stand for, are split finer where there are many of them, so that ragged
+// lengths spread evenly.  The choice changes no bit of the results.
+struct Share {      // one request's share of the items
+  Request x;
+  int tiles, blocks;
+  unsigned pieces, slots, items;
+  bool few;
+};
 struct Spans {
   unsigned span, fine;
 };
+__device__ __forceinline__ float load_of(const Share& s) {
+  return static_cast<float>(s.tiles) * static_cast<float>(s.blocks);
+}
 __device__ __forceinline__ Spans spans_of(const Params& p, float load) {
   load *= static_cast<float>(p.groups);
   const float t = static_cast<float>(p.target);
   return {static_cast<unsigned>(fmaxf(1.f, ceilf(load / t))),
-          static_cast<unsigned>(fmaxf(1.f, ceilf(load / (4.f * t))))};
+          static_cast<unsigned>(fmaxf(1.f, ceilf(load / (static_cast<float>(p.finer) * t))))};
 }
-__device__ __forceinline__ float load_of(const Params& p, const Request& x) {
-  return static_cast<float>(tiles_of(p, x)) * static_cast<float>(blocks_of(p, x));
+__device__ __forceinline__ Share share_of(const Params& p, int r) {
+  Share s;
+  s.x = r < p.R ? request(p, r) : Request{0, 0, 0};
+  s.tiles = tiles_of(p, s.x);
+  s.blocks = blocks_of(p, s.x);
+  s.few = min(s.x.n_tok, p.tile_tok) * p.group_heads <= p.fine_rows;
+  return s;
 }
-__device__ __forceinline__ unsigned pieces_of(const Params& p, const Request& x, const Spans& s,
-                                              int tiles, int blocks, unsigned& slots) {
-  const unsigned most = few_rows(p, x) ? s.fine : s.span;
-  const unsigned pieces = tiles == 0 ? 0 : max(1u, divide(blocks + most - 1, most));
-  const float want = static_cast<float>(x.n_tok) * static_cast<float>(p.H) *
-                     static_cast<float>(blocks);
-  slots = pieces <= 1 ? 0u : want >= static_cast<float>(kMuch) ? kMuch
-                                 : static_cast<unsigned>(x.n_tok) * p.H * blocks;
-  return pieces;
+// Pieces and the slots that the partial results of all its rows take.
+__device__ __forceinline__ void split_share(const Params& p, const Spans& sp, Share& s) {
+  const unsigned most = s.few ? sp.fine : sp.span;
+  s.pieces = s.tiles == 0 ? 0 : max(1u, divide(s.blocks + most - 1, most));
+  const float want = static_cast<float>(s.x.n_tok) * static_cast<float>(p.H) *
+                     static_cast<float>(s.blocks);
+  s.slots = s.pieces <= 1 ? 0u : want >= static_cast<float>(kMuch) ? kMuch
+                                     : static_cast<unsigned>(s.x.n_tok) * p.H * s.blocks;
+}
+// With `end` the slots up to its own: a request whose results do not fit is not split.
+__device__ __forceinline__ void count_items(const Params& p, unsigned end, Share& s) {
+  if (s.pieces > 1 && end > p.slots) s.pieces = 1;
+  s.items = s.tiles * s.pieces * p.groups;
+}
+// Its item number `in`.
+__device__ __forceinline__ Work work_of(const Params& p, int r, const Request& x, int tiles,
+                                        int blocks, unsigned pieces, unsigned base, unsigned in) {
+  const unsigned per_group = tiles * pieces;
+  Work w;
+  w.r = r;
+  w.pieces = pieces;
+  w.blocks = blocks;
+  w.base = base;
+  w.x = x;
+  w.group = divide(in, per_group);
+  const unsigned rest = in - w.group * per_group, q = divide(rest, pieces);
+  w.tile = tiles - 1 - static_cast<int>(q);
+  w.piece = rest - q * pieces;
+  w.kvh = p.by_group(w.group);
+  return w;
 }
 
-// One request's share of the search: its items are [at, at + items).
-template <int NT, int ITEMS>
-__device__ __forceinline__ void take_items(const Params& p, int item, SchedSmem<NT, ITEMS>& s,
-                                           int r, const Request& x, int tiles, int blocks,
-                                           unsigned pieces, unsigned base, unsigned at,
-                                           unsigned items) {
-#pragma unroll
-  for (int k = 0; k < ITEMS; ++k) {
-    const unsigned i = static_cast<unsigned>(item + k);
-    if (i < at || i >= at + items) continue;
-    const unsigned in = i - at, per_group = tiles * pieces;
-    Work w;
-    w.r = r;
-    w.pieces = pieces;
-    w.blocks = blocks;
-    w.base = base;
-    w.x = x;
-    w.group = divide(in, per_group);
-    const unsigned rest = in - w.group * per_group, q = divide(rest, pieces);
-    w.tile = tiles - 1 - static_cast<int>(q);
-    w.piece = rest - q * pieces;
-    w.kvh = p.by_group(w.group);
-    s.found[k] = w;
-    s.hit[k] = 1;
-  }
-}
+constexpr int kFewRequests = 64;
 
-// Finds the work of block `blk` of the call, with all threads of the block (NT); the answer is
-// in `s` after the block's next barrier (after __syncwarp for warp 0, if there are at most 64
-// requests).  Block b takes items ITEMS b ... of the call, or, as long as there are no more
-// items than `spread`, item b alone.  Items go request by request -- first the requests whose
-// tiles have many rows, whose items are the long ones -- in a request group of heads by group,
-// tile by tile from the last (in causal attention the longest) to the first, piece by piece of
-// a tile's keys.  Up to 64 requests one warp does it in registers; beyond, the block scans
-// them 32 a warp at a time.  The block that `publish`es leaves the split of every request for
-// the join.
-template <int NT, int ITEMS>
-__device__ __forceinline__ void find_work(const Params& p, int blk, int spread,
-                                          SchedSmem<NT, ITEMS>& s, bool publish) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (p.R <= 64) {
-    if (warp != 0) return;
-    if (lane < ITEMS) s.hit[lane] = 0;
-    __syncwarp();
-    const int halves = p.R > 32 ? 2 : 1;
-    Request x[2];
-    int tiles[2], blocks[2];
-    float load = 0.f;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = lane + 32 * h;
-      x[h] = r < p.R ? request(p, r) : Request{0, 0, 0};
-      tiles[h] = tiles_of(p, x[h]);
-      blocks[h] = blocks_of(p, x[h]);
-      load += static_cast<float>(tiles[h]) * static_cast<float>(blocks[h]);
+// One warp's view of the items.  Up to 64 requests it works them out by itself, two requests a
+// lane; beyond, schedule_kernel has left them in the workspace.
+struct Finder {
+  Share s[2];
+  unsigned base[2], at[2];
+  unsigned total;
+
+  __device__ __forceinline__ void begin(const Params& p, bool publish) {
+    if (p.R > kFewRequests) {
+      const int4 h = *p.head;
+      total = h.x + h.y;
+      return;
+    }
+    const int lane = threadIdx.x & 31;
+    s[0] = share_of(p, lane);
+    s[1] = share_of(p, p.R);  // none
+    float load = load_of(s[0]);
+    if (p.R > 32) {
+      s[1] = share_of(p, lane + 32);
+      load += load_of(s[1]);
     }
     const Spans sp = spans_of(p, warp_sum(load));
-    unsigned pieces[2] = {0, 0}, base[2], at[2], items[2];
     unsigned slots0 = 0, many0 = 0, few0 = 0, split = 0;
-    bool few[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      at[h] = base[h] = items[h] = 0;
-      few[h] = few_rows(p, x[h]);
-      if (h >= halves) continue;
-      unsigned slots;
-      pieces[h] = pieces_of(p, x[h], sp, tiles[h], blocks[h], slots);
-      unsigned none = 0, ends = slots;
-      if (__any_sync(0xffffffffu, slots != 0)) warp_scan(none, ends, lane);
-      base[h] = add_sat(slots0, ends) - slots;  // (exact below kMuch)
-      if (pieces[h] > 1 && add_sat(slots0, ends) > p.slots) pieces[h] = 1;  // no room for them
-      slots0 = add_sat(slots0, __shfl_sync(0xffffffffu, ends, 31));
-      items[h] = tiles[h] * pieces[h] * p.groups;
-      unsigned m = few[h] ? 0 : items[h], f = items[h] - m;
-      warp_scan(m, f, lane);
-      at[h] = few[h] ? few0 + f - items[h] : many0 + m - items[h];
+      base[h] = at[h] = 0;
+      s[h].items = s[h].pieces = 0;
+      if (h == 1 && p.R <= 32) continue;
+      split_share(p, sp, s[h]);
+      unsigned end = slots0;
+      if (__any_sync(0xffffffffu, s[h].slots != 0)) end = add_sat(slots0, warp_scan(s[h].slots));
+      base[h] = end - s[h].slots;
+      slots0 = __shfl_sync(0xffffffffu, end, 31);
+      count_items(p, end, s[h]);
+      split |= s[h].pieces > 1;
+      const unsigned m = warp_scan(s[h].few ? 0 : s[h].items);
+      const unsigned f = warp_scan(s[h].few ? s[h].items : 0);
+      at[h] = (s[h].few ? few0 + f : many0 + m) - s[h].items;
       many0 += __shfl_sync(0xffffffffu, m, 31);
       few0 += __shfl_sync(0xffffffffu, f, 31);
-      split |= pieces[h] > 1;
     }
-    const int per = many0 + few0 <= static_cast<unsigned>(spread) ? 1 : ITEMS;
+    total = many0 + few0;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      if (s[h].few) at[h] += many0;
       const int r = lane + 32 * h;
-      if (few[h]) at[h] += many0;
-      if (items[h] != 0) {
-        take_items(p, blk * per, s, r, x[h], tiles[h], blocks[h], pieces[h], base[h], at[h],
-                   items[h]);
-      }
-      if (publish && r < p.R) p.info[r] = make_int4(pieces[h], blocks[h], base[h], 0);
+      if (publish && r < p.R) p.info[r] = make_int4(s[h].pieces, s[h].blocks, base[h], 0);
     }
-    __syncwarp();
-    if (lane >= per && lane < ITEMS) s.hit[lane] = 0;
     if (publish) {
       split = __any_sync(0xffffffffu, split);
-      if (lane == 0) *p.any_split = split;
+      if (lane == 0) *p.head = make_int4(many0, few0, split, 0);
     }
-    return;
   }
-  if (tid < ITEMS) s.hit[tid] = 0;
-  float load = 0.f;
-  for (int r = tid; r < p.R; r += NT) load += load_of(p, request(p, r));
-  load = warp_sum(load);
-  if (lane == 0) s.f[warp] = load;
-  __syncthreads();
-  load = 0.f;
+
+  // Item i < total, to `out` (shared memory), by the whole warp.
+  __device__ __forceinline__ void find(const Params& p, unsigned i, Work* out) const {
+    const int lane = threadIdx.x & 31;
+    if (p.R <= kFewRequests) {
 #pragma unroll
-  for (int w = 0; w < NT / 32; ++w) load += s.f[w];
-  const Spans sp = spans_of(p, load);
-  // pass 0 counts the items, pass 1 places them
-  unsigned split = 0, many_all = 0;
-  int per = ITEMS;
-#pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {
-    unsigned many0 = 0, few0 = 0, slots0 = 0;
-#pragma unroll 1
-    for (int r0 = 0; r0 < p.R; r0 += NT) {
-      const int r = r0 + tid;
-      const Request x = r < p.R ? request(p, r) : Request{0, 0, 0};
-      const int tiles = tiles_of(p, x), blocks = blocks_of(p, x);
-      const bool few = few_rows(p, x);
-      unsigned slots, none = 0;
-      unsigned pieces = pieces_of(p, x, sp, tiles, blocks, slots);
-      unsigned ends = slots;
-      warp_scan(none, ends, lane);
-      if (lane == 31) s.b[warp] = ends;
-      __syncthreads();
-      unsigned total = 0;
-#pragma unroll
-      for (int w = 0; w < NT / 32; ++w) {
-        if (w == warp) ends = add_sat(ends, add_sat(slots0, total));
-        total = add_sat(total, s.b[w]);
-      }
-      slots0 = add_sat(slots0, total);
-      if (pieces > 1 && ends > p.slots) pieces = 1;  // no room for its partial results
-      const unsigned items = tiles * pieces * p.groups;
-      unsigned m = few ? 0 : items, f = items - m;
-      warp_scan(m, f, lane);
-      if (lane == 31) {
-        s.a[warp] = m;
-        s.c[warp] = f;
-      }
-      __syncthreads();
-      unsigned at = few ? few0 + f - items : many0 + m - items;
-#pragma unroll
-      for (int w = 0; w < NT / 32; ++w) {
-        if (w < warp) at += few ? s.c[w] : s.a[w];
-        many0 += s.a[w];
-        few0 += s.c[w];
-      }
-      if (pass == 1) {
-        if (few) at += many_all;
-        if (items != 0) {
-          take_items(p, blk * per, s, r, x, tiles, blocks, pieces, ends - slots, at, items);
+      for (int h = 0; h < 2; ++h) {
+        const Share& x = s[h];
+        if (i >= at[h] && i < at[h] + x.items) {
+          *out = work_of(p, lane + 32 * h, x.x, x.tiles, x.blocks, x.pieces, base[h], i - at[h]);
         }
-        if (publish && r < p.R) p.info[r] = make_int4(pieces, blocks, ends - slots, 0);
-        split |= pieces > 1;
       }
+      return;
     }
-    many_all = many0;
-    per = many0 + few0 <= static_cast<unsigned>(spread) ? 1 : ITEMS;
+    // the first request whose end lies behind the item, 32-way
+    const unsigned many = p.head->x;
+    const bool few = i >= many;
+    const unsigned v = few ? i - many : i;
+    int lo = 0, n = p.R;  // it is among [lo, lo + n)
+    while (n > 1) {
+      const int step = (n + 31) / 32;
+      const int last = min(lo + (lane + 1) * step, lo + n) - 1;  // of this lane's part
+      const int2 e = p.ends[last];
+      const unsigned behind =
+          __ballot_sync(0xffffffffu, static_cast<unsigned>(few ? e.y : e.x) > v);
+      const int k = __ffs(behind) - 1;  // (there is one: i < total)
+      const int start = lo + k * step;
+      n = min(step, lo + n - start);
+      lo = start;
+    }
+    if (lane == 0) {
+      const Share x = share_of(p, lo);
+      const int4 info = p.info[lo];
+      const unsigned items = x.tiles * info.x * p.groups;
+      const int2 e = p.ends[lo];
+      *out = work_of(p, lo, x.x, x.tiles, x.blocks, info.x, info.z,
+                     v - (static_cast<unsigned>(few ? e.y : e.x) - items));
+    }
   }
-  __syncthreads();
-  if (tid >= per && tid < ITEMS) s.hit[tid] = 0;
-  if (publish) {
-    split = __syncthreads_or(split);
-    if (tid == 0) *p.any_split = split;
-  }
-}
+};
 
 // Slot of the partial result of (row, block i of its tile's list).
 __device__ __forceinline__ int64_t part_slot(const Params& p, int base, int blocks,

@@ -115,7 +115,6 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
-// The four softmax warps of an item, or (both) those of the two items.
 // A whole warp's wait, bounded like mbar_wait; a loop of few instructions (the kernel's code
 // has to stay within the instruction cache: at 142 KB every step of it was fetched anew, and
 // the kernel ran no faster than its code came in).
@@ -145,13 +144,18 @@ __device__ __forceinline__ bool elect_one() {
   return yes != 0;
 }
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
-__device__ __forceinline__ void softmax_sync(int item, bool both) {
-  if (both) {
-    asm volatile("bar.sync 3, 256;" ::: "memory");
-  } else {
-    asm volatile("bar.sync %0, 128;" ::"r"(1 + item) : "memory");
-  }
+// A vote of an item's four softmax warps; and a barrier of both items'.
+__device__ __forceinline__ bool item_any(int item, bool vote) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\t"
+      "bar.red.or.pred q, %1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(1 + item), "r"(static_cast<uint32_t>(vote))
+      : "memory");
+  return any != 0;
 }
+__device__ __forceinline__ void both_sync() { asm volatile("bar.sync 3, 256;" ::: "memory"); }
 
 // Two fp32 numbers in one 64-bit register, two operations in one instruction, each rounded to
 // nearest.  (Constants are kept packed: a register short, the compiler would otherwise pack
@@ -254,8 +258,8 @@ __device__ __forceinline__ unsigned steps_of(const Params& p, const Item& it, in
   return set;
 }
 
-// Describes both items of the block, 16 lanes of a warp each.
-__device__ __forceinline__ void make_items(const Params& p, const SchedSmem<kThreads, 2>& s,
+// Describes the block's items (of which `there` exist), 16 lanes of a warp each.
+__device__ __forceinline__ void make_items(const Params& p, const Work (&found)[2], int there,
                                            bool shared, Item (&out)[2]) {
   const int lane = threadIdx.x & 15, k = (threadIdx.x & 31) >> 4;
   Item it;
@@ -264,8 +268,8 @@ __device__ __forceinline__ void make_items(const Params& p, const SchedSmem<kThr
   it.n_tok = it.rows = it.tok0 = it.pos0 = it.i0 = it.i1 = it.steps = 0;
   it.pmax = it.list_pos0 = it.list_pmax = -1;
   it.list = BlockList{0, 0, 0, 0};
-  if (s.hit[k]) {
-    const Work& w = s.found[k];
+  if (k < there) {
+    const Work& w = found[k];
     it.pieces = w.pieces;
     it.r = w.r;
     it.kvh = w.kvh;
@@ -281,8 +285,8 @@ __device__ __forceinline__ void make_items(const Params& p, const SchedSmem<kThr
     it.list_pos0 = it.pos0;
     it.list_pmax = it.pmax;
     if (shared) {  // item 1 is the tile before item 0's
-      it.list_pos0 = first + s.found[1].tile * p.tile_tok;
-      it.list_pmax = first + min((s.found[0].tile + 1) * p.tile_tok, w.x.n_tok) - 1;
+      it.list_pos0 = first + found[1].tile * p.tile_tok;
+      it.list_pmax = first + min((found[0].tile + 1) * p.tile_tok, w.x.n_tok) - 1;
     }
     it.list = block_list(p, it.list_pos0, it.list_pmax);
     it.i0 = piece_start(it.list.n, w.piece, w.pieces);
@@ -327,15 +331,15 @@ __device__ __forceinline__ int v_place(bool shared, int l0, int l1, int k, int j
 }
 
 struct Shared {
-  SchedSmem<kThreads, 2> sched;
+  Work found[2];
   uint64_t q_full[2], full[kMaxStages], empty[kMaxStages], s_full[2], p_half[2], p_ready[2],
       o_full[2], mma_done;
   uint32_t tmem;
   int abort_flag;
   int shared;             // the items share K and V
   Item item[2];
-  int keep_o[2];          // the softmax warps put values into O: accumulate on them
-  unsigned bad[2][2][4];  // keys of a step with a non-finite value that some row sees
+  int add[2];             // the item's next product is added to O (it does not start a key block)
+  unsigned bad[2][4];     // keys of a step with a non-finite value that some row sees
 };
 
 template <typename T, int D>
@@ -343,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     paged_tc_kernel(const __grid_constant__ CUtensorMap map_q,
                     const __grid_constant__ CUtensorMap map_q1,
                     const __grid_constant__ CUtensorMap map_k,
-                    const __grid_constant__ CUtensorMap map_v, const Params p, int n_sm) {
+                    const __grid_constant__ CUtensorMap map_v, const Params p) {
   using C = Cfg<D>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared sh;
@@ -367,7 +371,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sh.p_half[k], 4);
       mbar_init(&sh.p_ready[k], 4);
       mbar_init(&sh.o_full[k], 1);
-      sh.keep_o[k] = 0;
     }
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&sh.full[s], 1);
@@ -379,16 +382,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   grid_wait();
   grid_launch_dependents();
-  find_work<kThreads, 2>(p, blockIdx.x, n_sm, sh.sched, blockIdx.x == 0);
-  if (p.R > 64) __syncthreads();
   if (warp == 0) {
+    Finder finder;
+    finder.begin(p, blockIdx.x == 0);
+    // alone, as long as there is an SM for every item
+    const unsigned per = 2 * finder.total <= static_cast<unsigned>(p.target) ? 1 : 2;
+    const unsigned at = blockIdx.x * per;
+    const int there = at >= finder.total ? 0 : min(per, finder.total - at);
+#pragma unroll 1
+    for (int k = 0; k < there; ++k) finder.find(p, at + k, &sh.found[k]);
     __syncwarp();
     // two tiles of one request and group, their keys not split: they share K and V
-    const bool both = sh.sched.hit[0] && sh.sched.hit[1] &&
-                      sh.sched.found[0].r == sh.sched.found[1].r &&
-                      sh.sched.found[0].group == sh.sched.found[1].group &&
-                      sh.sched.found[0].pieces == 1;
-    make_items(p, sh.sched, both, sh.item);
+    const bool both = there == 2 && sh.found[0].r == sh.found[1].r &&
+                      sh.found[0].group == sh.found[1].group && sh.found[0].pieces == 1;
+    make_items(p, sh.found, there, both, sh.item);
     if (lane == 0) sh.shared = both;
   }
   __syncthreads();
@@ -492,8 +499,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t k_desc = umma_smem_desc(smem_u32(s_ring), 16, 1024, 2);
       // V (keys x D) is MN-major: 64-column slabs 16 KiB apart, 8-key groups 1 KiB
       const uint64_t v_desc = umma_smem_desc(smem_u32(s_ring), kTile * 128, 1024, 2);
-      StepIter it0{uniform(sh.item[0].i0), 0, 0}, it1{uniform(sh.item[1].i0), 0, 0};
-      unsigned fresh = 3;  // bit k: item k's next product starts a key block
       bool ok = true;
       int stage = 0;       // of the next tile of the ring ...
       uint32_t phase = 0;  // ... and its barrier's parity
@@ -523,36 +528,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (j >= steps || steps == 0) continue;
           int ks = stage;
           uint32_t kph = phase;
-          bool ends = false;  // the step ends its key block
+          const bool waited = both && k == 1;  // for its tiles, in item 0's turn
           if (j < 0) {
             ok = warp_wait(&sh.q_full[k], 0, abort_flag);
           } else {
             behind();
             ks = next;
             kph = next_phase;
-            StepIter it = k == 0 ? it0 : it1;
-            next_step(p, sh.item[k], it);
-            if (k == 0) it0 = it; else it1 = it;
-            ends = __shfl_sync(0xffffffffu, it.left == 0, 0);
-            ok = warp_wait(&sh.full[stage], phase, abort_flag);
+            if (!waited) ok = warp_wait(&sh.full[stage], phase, abort_flag);
           }
-          if (j + 1 < steps) ok = ok && warp_wait(&sh.full[ks], kph, abort_flag);
+          if (j + 1 < steps && !waited) ok = ok && warp_wait(&sh.full[ks], kph, abort_flag);
           if (j >= 0) {
             ok = ok && warp_wait(&sh.p_half[k], j & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
-            volatile int* keep = &sh.keep_o[k];
-            bool first = (fresh >> k) & 1u;
-            if (uniform(*keep)) {
-              first = false;
-              __syncwarp();
-              if (leader) *keep = 0;
-            }
+            const bool add = uniform(*const_cast<volatile int*>(&sh.add[k])) != 0;
             // keys 64..127 while the weights of keys 0..63 are still being computed
             const uint64_t vd = v_desc + stage * kTileUnits;
             const uint32_t d = tm + 256 * k;
             if (leader) {
-              umma_f16_ts(d + 128, d + 64 + 4 * 8, vd + 4 * (2048 >> 4), idesc_o, !first);
+              umma_f16_ts(d + 128, d + 64 + 4 * 8, vd + 4 * (2048 >> 4), idesc_o, add);
 #pragma unroll
               for (int i = 5; i < 8; ++i) {
                 umma_f16_ts(d + 128, d + 64 + i * 8, vd + i * (2048 >> 4), idesc_o, true);
@@ -571,7 +566,6 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (j + 1 == steps) umma_commit(&sh.o_full[k]);
             }
             __syncwarp();
-            fresh = ends ? fresh | (1u << k) : fresh & ~(1u << k);
             if (!both) advance();  // (now the K tile, if there is one)
           }
           if (!ok) break;
@@ -628,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
     float m = -INFINITY, l = 0.f;
     bool fresh = true, ok = true;  // fresh: the step starts a key block
-    int block = 0, scans = 0;
+    int block = 0;
     StepIter it{item.i0, 0, 0};
     // do all rows see every key of the step at t0?
     auto whole_for = [&](int t0, int pos0, int pmax) {
@@ -772,7 +766,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         base = m == -INFINITY ? 0.f : -m;
       }
       if (__builtin_expect(!list_whole, 0)) {
-        // V of this step: thread = key (of shared tiles each item's threads take a half)
+        // V of this step: thread = key
         const int place = v_place(shared, sh.item[0].steps, sh.item[1].steps, k, step);
         const int stage = place % C::kStages;
         ok = warp_wait(&sh.full[stage], (place / C::kStages) & 1, abort_flag);
@@ -780,40 +774,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint8_t* vrow = s_ring + stage * C::kTileBytes + row * 128;
         const int key = t0 + row;
         const bool seen = key <= item.list_pmax && (key >= item.list.lo_key || key < p.first);
-        // seen by every row: nothing to do.  By some: look for non-finite values.  By none: zeros.
+        // seen by every row: the product may have what it holds.  Else look for non-finite values,
+        // at first only look: both items' warps read the tile.
         const bool by_all = key <= item.list_pos0 &&
                             (p.window == INT32_MAX || key > item.list_pmax - p.window ||
                              key < p.first);
         constexpr uint32_t em = exp_mask<T>() * 0x10001u;           // both values' exponents
         constexpr uint32_t one = (exp_mask<T>() & -exp_mask<T>()) * 0x10001u;
-        constexpr int kChunks = C::kHalves * 8 / 2;
-        bool found = false;
-#pragma unroll 1
-        for (int part = shared ? k : 0; part < (shared ? k + 1 : 2); ++part) {
-          // 16-byte chunk c of a row sits at c ^ (row & 7) of its 128 bytes
-          auto chunk = [&](int c) {
-            const int at = part * kChunks + c;
-            return reinterpret_cast<uint4*>(vrow + (at >> 3) * (kTile * 128) +
-                                            (((at ^ row) & 7) << 4));
-          };
-          if (by_all) continue;
-          uint32_t hit = seen ? 0u : 0x8000u;
-          if (seen) {
-#pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
-              const uint4 x = *chunk(c);
-              // an exponent of all ones carries into the sign's place
-              hit |= ((x.x & em) + one) | ((x.y & em) + one) | ((x.z & em) + one) |
-                     ((x.w & em) + one);
-            }
-          }
-          if ((hit & 0x80008000u) == 0) continue;
-          found |= seen;
-#pragma unroll 1
+        constexpr int kChunks = C::kHalves * 8;
+        // 16-byte chunk c of a row sits at c ^ (row & 7) of its 128 bytes
+        auto chunk = [&](int c) {
+          return reinterpret_cast<uint4*>(vrow + (c >> 3) * (kTile * 128) + (((c ^ row) & 7) << 4));
+        };
+        uint32_t hit = 0;
+        if (!by_all) {
+#pragma unroll 4
           for (int c = 0; c < kChunks; ++c) {
-            uint4* at = chunk(c);
-            uint4 x = seen ? *at : make_uint4(0u, 0u, 0u, 0u);
-            if (seen) {
+            const uint4 x = *chunk(c);
+            // an exponent of all ones carries into the sign's place
+            hit |= ((x.x & em) + one) | ((x.y & em) + one) | ((x.z & em) + one) |
+                   ((x.w & em) + one);
+          }
+        }
+        const bool found = (hit & 0x80008000u) != 0;
+        const bool any = item_any(k, found);  // (both items' warps come to the same answer)
+        if (__builtin_expect(any, 0)) {
+          // Take them out, and add those that some rows see to these rows' results by hand.
+          if (shared) both_sync();  // both have looked
+          const unsigned flags = __ballot_sync(0xffffffffu, found && seen);
+          if (lane == 0) sh.bad[k][warp & 3] = flags;
+          if (found) {
+#pragma unroll 1
+            for (int c = 0; c < kChunks; ++c) {  // (of shared tiles both write the same)
+              uint4* at = chunk(c);
+              uint4 x = *at;
               uint32_t* xw = reinterpret_cast<uint32_t*>(&x);
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
@@ -821,23 +815,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (top & 0x8000u) xw[e] &= 0xffff0000u;
                 if (top & 0x80000000u) xw[e] &= 0xffffu;
               }
+              *at = x;
             }
-            *at = x;
           }
-        }
-        const unsigned flags = __ballot_sync(0xffffffffu, found);
-        const int buf = scans++ & 1;
-        if (lane == 0) sh.bad[buf][k][warp & 3] = flags;
-        fence_proxy_async_smem();  // the zeros, to the product's reads
-        softmax_sync(k, shared);
-        unsigned bad[4], any = 0;
+          fence_proxy_async_smem();  // the zeros, to the product's reads
+          if (shared) {
+            both_sync();
+          } else {
+            item_any(k, false);
+          }
+          unsigned bad[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          bad[b] = sh.bad[buf][k][b] | (shared ? sh.bad[buf][k ^ 1][b] : 0u);
-          any |= bad[b];
-        }
-        if (__builtin_expect(any != 0, 0)) {
-          // add the non-finite values to the rows that see them
+          for (int b = 0; b < 4; ++b) bad[b] = sh.bad[k][b];
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
             uint32_t o[32];
@@ -874,9 +863,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             tmem_st_x32(tO + c, o);
           }
-          if (row == 0) *const_cast<volatile int*>(&sh.keep_o[k]) = 1;
+          fresh = false;  // O holds values now
+          reload();
         }
-        reload();
       }
       uint64_t sum[2] = {0ull, 0ull};
       const uint64_t base2 = pair(base, base);
@@ -888,7 +877,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.p_half[k]);
+      if (lane == 0) {
+        if ((warp & 3) == 0) *const_cast<volatile int*>(&sh.add[k]) = !fresh;
+        mbar_arrive(&sh.p_half[k]);
+      }
       if (warp_live) {
         tmem_ld_wait(sa);
         tmem_ld_32x32b_x32(tS + 32, sb);
@@ -970,10 +962,9 @@ static int launch(const PagedSdpaArgs& a, const Params& p, int64_t items, cudaSt
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(paged_sdpa)");
   cudaLaunchConfig_t cfg = {};
-  // two items a block, or one while there are no more items than SMs
-  const int n_sm = device_sm_count();
-  cfg.gridDim = dim3(static_cast<unsigned>(std::max<int64_t>((items + 1) / 2,
-                                                             std::min<int64_t>(items, n_sm))));
+  // two items a block; no fewer blocks than SMs, for calls whose items each get their own
+  cfg.gridDim = dim3(static_cast<unsigned>(
+      std::max<int64_t>((items + 1) / 2, std::min<int64_t>(items, device_sm_count()))));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = stream;
@@ -982,7 +973,7 @@ static int launch(const PagedSdpaArgs& a, const Params& p, int64_t items, cudaSt
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, paged_tc_kernel<T, D>, mq, mq1, mk, mv, p, n_sm),
+  return cuda_status(cudaLaunchKernelEx(&cfg, paged_tc_kernel<T, D>, mq, mq1, mk, mv, p),
                      "paged_sdpa tensor-core launch");
 }
 
