@@ -184,11 +184,13 @@ __global__ void __launch_bounds__(kSimtThreads) paged_simt_kernel(const Params p
       const int row = warp * kSimtRows + r;
       if (w.pieces > 1) {
         if (row < rows) {
-          const int64_t at = part_slot(p, w.base, w.blocks, tok0 + row / heads,
-                                       head0 + row % heads, done);
-          if (lane == 0) p.part_ml[at] = make_float2(m[r], l[r]);
+          const Part at = part_of(p, w.x, w.base, w.blocks, w.tile, w.group, done);
+          if (lane == 0) p.part_ml[at.first + row] = make_float2(m[r], l[r]);
 #pragma unroll
-          for (int c = 0; c < DC; ++c) p.part_o[at * D + c * 32 + lane] = o[r][c];
+          for (int c = 0; c < DC; ++c) {
+            const int col = c * 32 + lane;
+            reinterpret_cast<float*>(part_at<D>(p, at, row, col & ~3))[col & 3] = o[r][c];
+          }
         }
       } else {
         float fa, fb;
@@ -378,31 +380,35 @@ __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const Params
 }
 
 // ---------------------------------------------------------------------------
-// Join of the partial results of split requests: a warp takes one row (token, head) and
-// folds its blocks' partial results in order, with the operations of the unsplit kernels.
-// Launched behind every call (the split is decided on the device); where nothing was split
-// it reads one word.  Its launch overlaps the main kernel's tail.
+// Join of the partial results of split requests: a warp takes two neighbouring heads of a token
+// (half of its lanes each, four columns at a time) and folds their blocks' partial results in
+// order, with the operations of the unsplit kernels.  Launched behind every call (the split is
+// decided on the device); where nothing was split it reads one word.  Its launch overlaps the
+// main kernel's tail.
 // ---------------------------------------------------------------------------
 constexpr int kJoinThreads = 128;
 
 template <typename T, int DC>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
   constexpr int D = 32 * DC;
-  constexpr int kAhead = 8;  // partial results in flight
+  constexpr int kQuads = (D / 4 + 15) / 16;  // of a lane's columns
+  constexpr int kAhead = 16 / kQuads;        // partial results in flight
   grid_wait();
   if (p.head->z == 0) return;
-  const int lane = threadIdx.x & 31;
-  const int64_t n_rows = static_cast<int64_t>(p.T) * p.H;
+  const int lane = threadIdx.x & 31, quad0 = lane >> 1;
+  const int h_pairs = (p.H + 1) / 2;
+  const int64_t n_pairs = static_cast<int64_t>(p.T) * h_pairs;
   const int64_t warps = static_cast<int64_t>(gridDim.x) * (kJoinThreads / 32);
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * (kJoinThreads / 32) + (threadIdx.x >> 5);
-       row < n_rows; row += warps) {
-    const int tok = static_cast<int>(row / p.H), head = static_cast<int>(row % p.H);
+  for (int64_t at = static_cast<int64_t>(blockIdx.x) * (kJoinThreads / 32) + (threadIdx.x >> 5);
+       at < n_pairs; at += warps) {
+    const int tok = static_cast<int>(at / h_pairs);
+    const int head = static_cast<int>(at - static_cast<int64_t>(tok) * h_pairs) * 2 + (lane & 1);
     // its request: the last one that starts at or before it (32-way search)
     int lo = 0, hi = p.R;  // answer + 1 is in (lo, hi]
     while (hi - lo > 1) {
       const int step = (hi - lo + 31) / 32;
-      const int at = lo + lane * step;
-      const bool le = at < hi && clampi(p.query_start[at], 0, p.T) <= tok;
+      const int i = lo + lane * step;
+      const bool le = i < hi && clampi(p.query_start[i], 0, p.T) <= tok;
       const unsigned bal = __ballot_sync(0xffffffffu, le);
       if (bal == 0) break;
       const int k = 31 - __clz(bal);
@@ -411,27 +417,36 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     }
     const int r = lo;
     const Request x = request(p, r);
-    if (tok < x.tok || tok >= x.tok + x.n_tok) continue;
     const int4 info = p.info[r];
-    if (info.x <= 1) continue;
-    const int in = tok - x.tok, tile = p.by_tile(in);
-    const int pos0 = x.seq - x.n_tok + tile * p.tile_tok;
-    const int n_tok = min(p.tile_tok, x.n_tok - tile * p.tile_tok);
+    if (tok < x.tok || tok >= x.tok + x.n_tok || info.x <= 1) continue;
+    if (head >= p.H) continue;
+    const int in = tok - x.tok, tile = p.by_tile(in), first = tile * p.tile_tok;
+    const int pos0 = x.seq - x.n_tok + first;
+    const int n_tok = min(p.tile_tok, x.n_tok - first);
     const BlockList list = block_list(p, pos0, pos0 + n_tok - 1);
-    const int64_t at = part_slot(p, info.z, info.y, in, head, 0);
-    float m = -INFINITY, l = 0.f, o[DC];
+    // its group of heads and its row in the tile, whose rows are tokens x the group's heads
+    const int kvh = head / p.G, in_kv = head - kvh * p.G, sub = in_kv / p.group_heads;
+    const int group = kvh * (p.groups / p.Hkv) + sub;
+    const int heads = min(p.group_heads, p.G - sub * p.group_heads);
+    const int row = (in - first) * heads + in_kv - sub * p.group_heads;
+    const Part part = part_of(p, x, info.z, info.y, tile, group, 0);
+    float m = -INFINITY, l = 0.f;
+    float4 o[kQuads];
 #pragma unroll
-    for (int c = 0; c < DC; ++c) o[c] = 0.f;
+    for (int c = 0; c < kQuads; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i = 0; i < list.n; i += kAhead) {
       float2 ml[kAhead];
-      float po[kAhead][DC];
+      float4 po[kAhead][kQuads];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        const bool in_list = i + j < list.n;
-        ml[j] = in_list ? p.part_ml[at + i + j] : make_float2(-INFINITY, 0.f);
+        const bool there = i + j < list.n;
+        const Part b = {part.first + static_cast<int64_t>(i + j) * part.rows, part.rows};
+        ml[j] = there ? p.part_ml[b.first + row] : make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (int c = 0; c < DC; ++c) {
-          po[j][c] = in_list ? p.part_o[(at + i + j) * D + c * 32 + lane] : 0.f;
+        for (int c = 0; c < kQuads; ++c) {
+          const int col = 4 * (quad0 + 16 * c);
+          po[j][c] = there && col < D ? *part_at<D>(p, b, row, col)
+                                      : make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
 #pragma unroll
@@ -440,14 +455,30 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
         fold_factors(m, ml[j].x, fa, fb);
         l = fold_value(l, ml[j].y, fa, fb);
 #pragma unroll
-        for (int c = 0; c < DC; ++c) o[c] = fold_value(o[c], po[j][c], fa, fb);
+        for (int c = 0; c < kQuads; ++c) {
+          o[c].x = fold_value(o[c].x, po[j][c].x, fa, fb);
+          o[c].y = fold_value(o[c].y, po[j][c].y, fa, fb);
+          o[c].z = fold_value(o[c].z, po[j][c].z, fa, fb);
+          o[c].w = fold_value(o[c].w, po[j][c].w, fa, fb);
+        }
       }
     }
     const float sink = p.sinks ? to_f32(static_cast<const T*>(p.sinks)[head]) * kLog2e : 0.f;
     const float sc = row_scale(m, l, p.sinks != nullptr, sink);
     T* dst = static_cast<T*>(p.out) + tok * p.os[0] + head * p.os[1];
 #pragma unroll
-    for (int c = 0; c < DC; ++c) dst[c * 32 + lane] = from_f32<T>(row_value(o[c], sc));
+    for (int c = 0; c < kQuads; ++c) {
+      const int col = 4 * (quad0 + 16 * c);
+      if (col >= D) continue;
+      struct alignas(4 * sizeof(T)) Quad {
+        T v[4];
+      } q;
+      q.v[0] = from_f32<T>(row_value(o[c].x, sc));
+      q.v[1] = from_f32<T>(row_value(o[c].y, sc));
+      q.v[2] = from_f32<T>(row_value(o[c].z, sc));
+      q.v[3] = from_f32<T>(row_value(o[c].w, sc));
+      *reinterpret_cast<Quad*>(dst + col) = q;
+    }
   }
 }
 
@@ -482,8 +513,8 @@ static int launch_simt(const Params& p, int64_t items, cudaStream_t stream) {
 }
 template <typename T, int DC>
 static int launch_join(const Params& p, cudaStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(p.T) * p.H;
-  const int64_t want = (rows + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
+  const int64_t pairs = static_cast<int64_t>(p.T) * ((p.H + 1) / 2);
+  const int64_t want = (pairs + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
   const unsigned grid =
       static_cast<unsigned>(std::min<int64_t>(want, 8LL * device_sm_count()));
   return cuda_status(launch_early(join_kernel<T, DC>, grid, kJoinThreads, 0, stream, p),

@@ -105,7 +105,7 @@ struct Params {
   int4* info;              // per request {pieces, blocks a row has, first slot, -}
   int2* ends;              // per request {items of many rows up to its own, of few rows}
   float2* part_ml;         // (slot,) (m, l)
-  float* part_o;           // (slot, D)
+  float* part_o;           // D columns a slot (see Part)
   unsigned slots;
 };
 
@@ -241,10 +241,11 @@ __device__ __forceinline__ Share share_of(const Params& p, int r) {
 __device__ __forceinline__ void split_share(const Params& p, const Spans& sp, Share& s) {
   const unsigned most = s.few ? sp.fine : sp.span;
   s.pieces = s.tiles == 0 ? 0 : max(1u, divide(s.blocks + most - 1, most));
-  const float want = static_cast<float>(s.x.n_tok) * static_cast<float>(p.H) *
-                     static_cast<float>(s.blocks);
+  const unsigned rows = min(s.x.n_tok, p.tile_tok) * p.group_heads;  // as in part_of
+  const float want = static_cast<float>(s.tiles) * static_cast<float>(p.groups) *
+                     static_cast<float>(s.blocks) * static_cast<float>(rows);
   s.slots = s.pieces <= 1 ? 0u : want >= static_cast<float>(kMuch) ? kMuch
-                                     : static_cast<unsigned>(s.x.n_tok) * p.H * s.blocks;
+                                     : static_cast<unsigned>(s.tiles) * p.groups * s.blocks * rows;
 }
 // With `end` the slots up to its own: a request whose results do not fit is not split.
 __device__ __forceinline__ void count_items(const Params& p, unsigned end, Share& s) {
@@ -365,10 +366,30 @@ struct Finder {
   }
 };
 
-// Slot of the partial result of (row, block i of its tile's list).
-__device__ __forceinline__ int64_t part_slot(const Params& p, int base, int blocks,
-                                             int tok_in_request, int head, int i) {
-  return base + (static_cast<int64_t>(tok_in_request) * p.H + head) * blocks + i;
+// Where the partial results of block i of a tile's list are, of which a request keeps `rows` per
+// tile and block: first the place of row 0's (m, l) and of its columns.  Columns lie four by
+// four, a row's four next to the other rows', so that a warp with a row per lane stores (and the
+// join, with a few rows per warp, reads) whole sectors: row by row, 64 KiB took a block 9000
+// clocks to leave.
+struct Part {
+  int64_t first;
+  int rows;
+};
+__device__ __forceinline__ int part_rows(const Params& p, const Request& x) {
+  return min(x.n_tok, p.tile_tok) * p.group_heads;
+}
+__device__ __forceinline__ Part part_of(const Params& p, const Request& x, unsigned base,
+                                        int blocks, int tile, int group, int i) {
+  const int rows = part_rows(p, x);
+  return {static_cast<int64_t>(base) +
+              (static_cast<int64_t>(tile * p.groups + group) * blocks + i) * rows,
+          rows};
+}
+// Column col (a multiple of 4) of `row`.
+template <int D>
+__device__ __forceinline__ float4* part_at(const Params& p, const Part& a, int row, int col) {
+  return reinterpret_cast<float4*>(p.part_o) + a.first * (D / 4) +
+         static_cast<int64_t>(col / 4) * a.rows + row;
 }
 
 __device__ __forceinline__ void grid_launch_dependents() {

@@ -236,7 +236,8 @@ __device__ __forceinline__ void weights_of(const uint32_t (&s)[32], uint64_t sca
 // What one of a block's two items is.
 struct Item {
   int pieces;             // 0: it is not there
-  int r, kvh, tok, base, blocks;  // request, KV head, first row, Work's base and blocks
+  int r, kvh, tok;        // request, KV head, first row
+  Part part;              // its partial results, of the list's first block (pieces > 1)
   int n_tok, rows, tok0;  // its tile (tok0 in the request)
   int pos0, pmax;         // positions of its first and last token
   // the keys it walks: blocks [i0, i1) of `list`.  Items that share K and V walk the keys that
@@ -264,7 +265,8 @@ __device__ __forceinline__ void make_items(const Params& p, const Work (&found)[
   const int lane = threadIdx.x & 15, k = (threadIdx.x & 31) >> 4;
   Item it;
   it.pieces = 0;
-  it.r = it.kvh = it.tok = it.base = it.blocks = 0;
+  it.r = it.kvh = it.tok = 0;
+  it.part = Part{0, 0};
   it.n_tok = it.rows = it.tok0 = it.pos0 = it.i0 = it.i1 = it.steps = 0;
   it.pmax = it.list_pos0 = it.list_pmax = -1;
   it.list = BlockList{0, 0, 0, 0};
@@ -273,8 +275,7 @@ __device__ __forceinline__ void make_items(const Params& p, const Work (&found)[
     it.pieces = w.pieces;
     it.r = w.r;
     it.kvh = w.kvh;
-    it.base = w.base;
-    it.blocks = w.blocks;
+    it.part = part_of(p, w.x, w.base, w.blocks, w.tile, w.group, 0);
     it.tok0 = w.tile * p.tile_tok;
     it.tok = w.x.tok + it.tok0;
     it.n_tok = min(p.tile_tok, w.x.n_tok - it.tok0);
@@ -633,20 +634,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     // items) left for the join.
     auto close_block = [&](float bm, float bl) {
       if (pieces > 1) {
-        const int64_t at = part_slot(p, item.base, item.blocks, item.tok0 + tok, head,
-                                     item.i0 + block);
-        if (live) p.part_ml[at] = make_float2(bm, bl);
+        const Part at = {item.part.first + static_cast<int64_t>(item.i0 + block) * item.part.rows,
+                         item.part.rows};
+        if (live) p.part_ml[at.first + row] = make_float2(bm, bl);
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           uint32_t o[32];
           tmem_ld_32x32b_x32(tO + c, o);
           tmem_ld_wait(o);
           if (live) {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + c);
+            float4* dst = part_at<D>(p, at, row, c);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              dst[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]),
-                                   __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
+              dst[static_cast<int64_t>(j) * at.rows] =
+                  make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]),
+                              __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
             }
           }
         }
