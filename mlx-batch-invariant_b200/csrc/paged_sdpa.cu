@@ -380,46 +380,66 @@ __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const Params
 }
 
 // ---------------------------------------------------------------------------
-// Join of the partial results of split requests: a warp takes two neighbouring heads of a token
-// (half of its lanes each, four columns at a time) and folds their blocks' partial results in
-// order, with the operations of the unsplit kernels.  Launched behind every call (the split is
-// decided on the device); where nothing was split it reads one word.  Its launch overlaps the
-// main kernel's tail.
+// Join of the partial results of split requests: a warp takes 64 columns of two neighbouring
+// heads of a token (half of its lanes each, four columns a lane) and folds their blocks' partial
+// results in order, with the operations of the unsplit kernels; 16 blocks' are in flight at a
+// time.  (A warp with all 128 columns had room for 8, and took 3 us longer where a token has 16
+// blocks.)  Launched behind every call (the split is decided on the device); where nothing was
+// split it reads one word.  Its launch overlaps the main kernel's tail.
 // ---------------------------------------------------------------------------
 constexpr int kJoinThreads = 128;
 
 template <typename T, int DC>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
   constexpr int D = 32 * DC;
-  constexpr int kQuads = (D / 4 + 15) / 16;  // of a lane's columns
-  constexpr int kAhead = 16 / kQuads;        // partial results in flight
+  constexpr int kParts = (D + 63) / 64;  // of a row's columns
+  constexpr int kAhead = 16;             // partial results in flight
   grid_wait();
-  if (p.head->z == 0) return;
-  const int lane = threadIdx.x & 31, quad0 = lane >> 1;
+  const int lane = threadIdx.x & 31;
+  // Up to 32 requests: each lane has one, so that what follows waits for memory once.
+  const bool small = p.R <= 32;
+  const int4 notes = *p.head;
+  const Request mine = small && lane < p.R ? request(p, lane) : Request{0, 0, 0};
+  const int4 my_info = small && lane < p.R ? p.info[lane] : make_int4(0, 0, 0, 0);
+  if (notes.z == 0) return;
   const int h_pairs = (p.H + 1) / 2;
-  const int64_t n_pairs = static_cast<int64_t>(p.T) * h_pairs;
+  const int64_t n_pairs = static_cast<int64_t>(p.T) * h_pairs * kParts;
   const int64_t warps = static_cast<int64_t>(gridDim.x) * (kJoinThreads / 32);
   for (int64_t at = static_cast<int64_t>(blockIdx.x) * (kJoinThreads / 32) + (threadIdx.x >> 5);
        at < n_pairs; at += warps) {
-    const int tok = static_cast<int>(at / h_pairs);
-    const int head = static_cast<int>(at - static_cast<int64_t>(tok) * h_pairs) * 2 + (lane & 1);
-    // its request: the last one that starts at or before it (32-way search)
-    int lo = 0, hi = p.R;  // answer + 1 is in (lo, hi]
-    while (hi - lo > 1) {
-      const int step = (hi - lo + 31) / 32;
-      const int i = lo + lane * step;
-      const bool le = i < hi && clampi(p.query_start[i], 0, p.T) <= tok;
-      const unsigned bal = __ballot_sync(0xffffffffu, le);
-      if (bal == 0) break;
-      const int k = 31 - __clz(bal);
-      lo = lo + k * step;
-      hi = min(hi, lo + step);
+    const int64_t pair = at / kParts;
+    const int col = 64 * static_cast<int>(at - pair * kParts) + 4 * (lane >> 1);
+    const int tok = static_cast<int>(pair / h_pairs);
+    const int head = static_cast<int>(pair - static_cast<int64_t>(tok) * h_pairs) * 2 + (lane & 1);
+    Request x;
+    int4 info;
+    if (small) {
+      const unsigned has = __ballot_sync(0xffffffffu, tok >= mine.tok && tok < mine.tok + mine.n_tok);
+      const int r = has != 0 ? __ffs(has) - 1 : 0;
+      x.tok = __shfl_sync(0xffffffffu, mine.tok, r);
+      x.n_tok = __shfl_sync(0xffffffffu, mine.n_tok, r);
+      x.seq = __shfl_sync(0xffffffffu, mine.seq, r);
+      info.x = __shfl_sync(0xffffffffu, my_info.x, r);
+      info.y = __shfl_sync(0xffffffffu, my_info.y, r);
+      info.z = __shfl_sync(0xffffffffu, my_info.z, r);
+    } else {
+      // its request: the last one that starts at or before it (32-way search)
+      int lo = 0, hi = p.R;  // answer + 1 is in (lo, hi]
+      while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32;
+        const int i = lo + lane * step;
+        const bool le = i < hi && clampi(p.query_start[i], 0, p.T) <= tok;
+        const unsigned bal = __ballot_sync(0xffffffffu, le);
+        if (bal == 0) break;
+        const int k = 31 - __clz(bal);
+        lo = lo + k * step;
+        hi = min(hi, lo + step);
+      }
+      x = request(p, lo);
+      info = p.info[lo];
     }
-    const int r = lo;
-    const Request x = request(p, r);
-    const int4 info = p.info[r];
     if (tok < x.tok || tok >= x.tok + x.n_tok || info.x <= 1) continue;
-    if (head >= p.H) continue;
+    if (head >= p.H || col >= D) continue;
     const int in = tok - x.tok, tile = p.by_tile(in), first = tile * p.tile_tok;
     const int pos0 = x.seq - x.n_tok + first;
     const int n_tok = min(p.tile_tok, x.n_tok - first);
@@ -431,54 +451,38 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     const int row = (in - first) * heads + in_kv - sub * p.group_heads;
     const Part part = part_of(p, x, info.z, info.y, tile, group, 0);
     float m = -INFINITY, l = 0.f;
-    float4 o[kQuads];
-#pragma unroll
-    for (int c = 0; c < kQuads; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i = 0; i < list.n; i += kAhead) {
       float2 ml[kAhead];
-      float4 po[kAhead][kQuads];
+      float4 po[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         const bool there = i + j < list.n;
         const Part b = {part.first + static_cast<int64_t>(i + j) * part.rows, part.rows};
         ml[j] = there ? p.part_ml[b.first + row] : make_float2(-INFINITY, 0.f);
-#pragma unroll
-        for (int c = 0; c < kQuads; ++c) {
-          const int col = 4 * (quad0 + 16 * c);
-          po[j][c] = there && col < D ? *part_at<D>(p, b, row, col)
-                                      : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+        po[j] = there ? *part_at<D>(p, b, row, col) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         float fa, fb;
         fold_factors(m, ml[j].x, fa, fb);
         l = fold_value(l, ml[j].y, fa, fb);
-#pragma unroll
-        for (int c = 0; c < kQuads; ++c) {
-          o[c].x = fold_value(o[c].x, po[j][c].x, fa, fb);
-          o[c].y = fold_value(o[c].y, po[j][c].y, fa, fb);
-          o[c].z = fold_value(o[c].z, po[j][c].z, fa, fb);
-          o[c].w = fold_value(o[c].w, po[j][c].w, fa, fb);
-        }
+        o.x = fold_value(o.x, po[j].x, fa, fb);
+        o.y = fold_value(o.y, po[j].y, fa, fb);
+        o.z = fold_value(o.z, po[j].z, fa, fb);
+        o.w = fold_value(o.w, po[j].w, fa, fb);
       }
     }
     const float sink = p.sinks ? to_f32(static_cast<const T*>(p.sinks)[head]) * kLog2e : 0.f;
     const float sc = row_scale(m, l, p.sinks != nullptr, sink);
-    T* dst = static_cast<T*>(p.out) + tok * p.os[0] + head * p.os[1];
-#pragma unroll
-    for (int c = 0; c < kQuads; ++c) {
-      const int col = 4 * (quad0 + 16 * c);
-      if (col >= D) continue;
-      struct alignas(4 * sizeof(T)) Quad {
-        T v[4];
-      } q;
-      q.v[0] = from_f32<T>(row_value(o[c].x, sc));
-      q.v[1] = from_f32<T>(row_value(o[c].y, sc));
-      q.v[2] = from_f32<T>(row_value(o[c].z, sc));
-      q.v[3] = from_f32<T>(row_value(o[c].w, sc));
-      *reinterpret_cast<Quad*>(dst + col) = q;
-    }
+    struct alignas(4 * sizeof(T)) Quad {
+      T v[4];
+    } q;
+    q.v[0] = from_f32<T>(row_value(o.x, sc));
+    q.v[1] = from_f32<T>(row_value(o.y, sc));
+    q.v[2] = from_f32<T>(row_value(o.z, sc));
+    q.v[3] = from_f32<T>(row_value(o.w, sc));
+    *reinterpret_cast<Quad*>(static_cast<T*>(p.out) + tok * p.os[0] + head * p.os[1] + col) = q;
   }
 }
 
@@ -513,7 +517,7 @@ static int launch_simt(const Params& p, int64_t items, cudaStream_t stream) {
 }
 template <typename T, int DC>
 static int launch_join(const Params& p, cudaStream_t stream) {
-  const int64_t pairs = static_cast<int64_t>(p.T) * ((p.H + 1) / 2);
+  const int64_t pairs = static_cast<int64_t>(p.T) * ((p.H + 1) / 2) * ((DC + 1) / 2);
   const int64_t want = (pairs + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
   const unsigned grid =
       static_cast<unsigned>(std::min<int64_t>(want, 8LL * device_sm_count()));
@@ -593,7 +597,8 @@ int launch_paged_sdpa(const PagedSdpaArgs& a, cudaStream_t stream) {
   p.n_pages = static_cast<int>(a.n_pages);
   p.page = static_cast<int>(a.page);
   p.shift = tc ? kTcShift : kSimtShift;
-  p.max_seq = std::min<int64_t>(a.width * a.page, INT32_MAX - (1 << kTcShift));
+  p.max_seq = static_cast<int>(
+      std::min<int64_t>(a.width * a.page, INT32_MAX - (1 << kTcShift)));
   p.group_heads = std::min(p.G, rows);
   p.tile_tok = rows / p.group_heads;
   const int subs = (p.G + rows - 1) / rows;

@@ -92,7 +92,7 @@ struct Params {
   int first;
   int T, R, H, Hkv, G;     // G = H / Hkv
   int n_pages, page;
-  int64_t max_seq;         // tokens a row of the block table holds
+  int max_seq;             // tokens a row of the block table holds
   int shift;               // log 2 of the keys of a block
   int tile_tok;            // tokens of a tile
   int groups, group_heads; // a KV head's query heads as groups (tiles cover one group)
@@ -158,10 +158,11 @@ struct Request {
   int seq;         // tokens of its sequence, the new ones among them
 };
 __device__ __forceinline__ Request request(const Params& p, int r) {
+  const int start = p.query_start[r], end = p.query_start[r + 1], seq = p.seq_lens[r];
   Request x;
-  x.tok = clampi(p.query_start[r], 0, p.T);
-  x.n_tok = clampi(p.query_start[r + 1], x.tok, p.T) - x.tok;
-  x.seq = clampi(p.seq_lens[r], 0, p.max_seq);
+  x.tok = min(max(start, 0), p.T);
+  x.n_tok = min(max(end, x.tok), p.T) - x.tok;
+  x.seq = min(max(seq, 0), p.max_seq);
   return x;
 }
 __device__ __forceinline__ int tiles_of(const Params& p, const Request& x) {
@@ -226,7 +227,7 @@ __device__ __forceinline__ float load_of(const Share& s) {
 __device__ __forceinline__ Spans spans_of(const Params& p, float load) {
   load *= static_cast<float>(p.groups);
   const float t = static_cast<float>(p.target);
-  return {static_cast<unsigned>(fmaxf(1.f, ceilf(load / t))),
+  return {static_cast<unsigned>(fmaxf(1.f, ceilf(2.f * load / t))),
           static_cast<unsigned>(fmaxf(1.f, ceilf(load / (static_cast<float>(p.finer) * t))))};
 }
 __device__ __forceinline__ Share share_of(const Params& p, int r) {

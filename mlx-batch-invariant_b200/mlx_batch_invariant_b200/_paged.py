@@ -27,7 +27,7 @@ from . import _lib
 from ._gemm import _check_cuda
 
 MAX_PAGED_HEAD_DIM = 256
-_short = _lib.short_way
+_new_tuple = tuple.__new__
 
 
 class PagedPlan(NamedTuple):
@@ -76,10 +76,10 @@ def paged_plan(query_lens, context_lens, block_table, page_size, num_tokens, *, 
     """
     compiling = torch.compiler.is_compiling()
     if not compiling:
-        out = _short().plan(query_lens, context_lens, block_table, page_size, num_tokens,
+        out = (_lib._short or _lib.short_way()).plan(query_lens, context_lens, block_table, page_size, num_tokens,
                             free_pages, free_head)
         if out.__class__ is tuple:
-            return PagedPlan._make(out)
+            return _new_tuple(PagedPlan, out)
         if out is not None:
             _lib.check(out, "bi_paged_plan")
     page_size, num_tokens = int(page_size), int(num_tokens)
@@ -179,7 +179,7 @@ def rope_kv_paged(qkv, cos, sin, positions, slots, k_cache, v_cache, *, out=None
     """
     compiling = torch.compiler.is_compiling()
     if not compiling:
-        q = _short().rope(qkv, cos, sin, positions, slots, k_cache, v_cache, out)
+        q = (_lib._short or _lib.short_way()).rope(qkv, cos, sin, positions, slots, k_cache, v_cache, out)
         if q.__class__ is not int and q is not None:
             return q
         if q is not None:
@@ -252,7 +252,7 @@ def paged_attention(q, k_cache, v_cache, block_table, query_start, seq_lens, *, 
     """
     compiling = torch.compiler.is_compiling()
     if not compiling:
-        o = _short().attention(q, k_cache, v_cache, block_table, query_start, seq_lens, scale,
+        o = (_lib._short or _lib.short_way()).attention(q, k_cache, v_cache, block_table, query_start, seq_lens, scale,
                                window, first_tokens, sinks, out)
         if o.__class__ is not int and o is not None:
             return o
