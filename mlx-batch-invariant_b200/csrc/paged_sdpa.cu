@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kSimtThreads) paged_simt_kernel(const Params p
       const int row = warp * kSimtRows + r;
       if (w.pieces > 1) {
         if (row < rows) {
-          const Part at = part_of(p, w.x, w.base, w.blocks, w.tile, w.group, done);
+          const Part at = part_of(p, w.x, w.base, w.entries, w.tile, w.group, done);
           if (lane == 0) p.part_ml[at.first + row] = make_float2(m[r], l[r]);
 #pragma unroll
           for (int c = 0; c < DC; ++c) {
@@ -369,7 +369,8 @@ __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const Params
     many0 += __shfl_sync(0xffffffffu, m, 31);
     few0 += __shfl_sync(0xffffffffu, f, 31);
     if (r < p.R) {
-      p.info[r] = make_int4(s.pieces, s.blocks, end - s.slots, 0);
+      const int entries = s.pieces > 1 ? entries_of(s.blocks, s.pieces, s.few) : 0;
+      p.info[r] = make_int4(s.pieces, entries, end - s.slots, 0);
       p.ends[r] = make_int2(m_end, f_end);
     }
     split |= s.pieces > 1;
@@ -450,14 +451,15 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     const int heads = min(p.group_heads, p.G - sub * p.group_heads);
     const int row = (in - first) * heads + in_kv - sub * p.group_heads;
     const Part part = part_of(p, x, info.z, info.y, tile, group, 0);
+    const int entries = entries_of(list.n, info.x, is_few(p, x));
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = 0; i < list.n; i += kAhead) {
+    for (int i = 0; i < entries; i += kAhead) {
       float2 ml[kAhead];
       float4 po[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        const bool there = i + j < list.n;
+        const bool there = i + j < entries;
         const Part b = {part.first + static_cast<int64_t>(i + j) * part.rows, part.rows};
         ml[j] = there ? p.part_ml[b.first + row] : make_float2(-INFINITY, 0.f);
         po[j] = there ? *part_at<D>(p, b, row, col) : make_float4(0.f, 0.f, 0.f, 0.f);

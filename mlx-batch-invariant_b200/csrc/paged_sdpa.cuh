@@ -102,7 +102,7 @@ struct Params {
   int finer;               // ... so many times finer
   // partial results of split requests
   int4* head;              // {items of many rows, of few rows, whether a request is split, -}
-  int4* info;              // per request {pieces, blocks a row has, first slot, -}
+  int4* info;              // per request {pieces, partial results a row has, first slot, -}
   int2* ends;              // per request {items of many rows up to its own, of few rows}
   float2* part_ml;         // (slot,) (m, l)
   float* part_o;           // D columns a slot (see Part)
@@ -177,10 +177,26 @@ __device__ __forceinline__ int blocks_of(const Params& p, const Request& x) {
   return static_cast<int>(most < all ? most : all);
 }
 
+// A tile of few rows: cheap to split, as its partial results are small beside the keys that
+// they stand for.
+__device__ __forceinline__ bool is_few(const Params& p, const Request& x) {
+  return min(x.n_tok, p.tile_tok) * p.group_heads <= p.fine_rows;
+}
+// Partial results that a tile of n blocks in `pieces` pieces leaves: one a block, but a tile of
+// many rows joins its first piece's blocks, the first in order, as it goes (their 64 KiB each
+// cost as much as the products: 128 tokens behind 30000, 329 -> 294 us).
+__device__ __forceinline__ int entries_of(int n, int pieces, bool few) {
+  return few || n == 0 ? n : n - piece_start(n, 1, pieces) + 1;
+}
+// The first one of piece `piece`, whose first block is i0.
+__device__ __forceinline__ int first_entry(int n, int piece, int pieces, bool few, int i0) {
+  return few || piece == 0 ? i0 : i0 - piece_start(n, 1, pieces) + 1;
+}
+
 struct Work {
   int r, tile, group, kvh, piece, pieces;
-  int blocks;        // most blocks a row of the request has
-  int base;          // first slot of the request's partial results (pieces > 1)
+  int entries;       // most partial results a row of the request has ...
+  int base;          // ... and their first slot (pieces > 1)
   Request x;
 };
 
@@ -227,7 +243,7 @@ __device__ __forceinline__ float load_of(const Share& s) {
 __device__ __forceinline__ Spans spans_of(const Params& p, float load) {
   load *= static_cast<float>(p.groups);
   const float t = static_cast<float>(p.target);
-  return {static_cast<unsigned>(fmaxf(1.f, ceilf(2.f * load / t))),
+  return {load <= t ? 1u : static_cast<unsigned>(ceilf(2.f * load / t)),
           static_cast<unsigned>(fmaxf(1.f, ceilf(load / (static_cast<float>(p.finer) * t))))};
 }
 __device__ __forceinline__ Share share_of(const Params& p, int r) {
@@ -235,7 +251,7 @@ __device__ __forceinline__ Share share_of(const Params& p, int r) {
   s.x = r < p.R ? request(p, r) : Request{0, 0, 0};
   s.tiles = tiles_of(p, s.x);
   s.blocks = blocks_of(p, s.x);
-  s.few = min(s.x.n_tok, p.tile_tok) * p.group_heads <= p.fine_rows;
+  s.few = is_few(p, s.x);
   return s;
 }
 // Pieces and the slots that the partial results of all its rows take.
@@ -243,10 +259,11 @@ __device__ __forceinline__ void split_share(const Params& p, const Spans& sp, Sh
   const unsigned most = s.few ? sp.fine : sp.span;
   s.pieces = s.tiles == 0 ? 0 : max(1u, divide(s.blocks + most - 1, most));
   const unsigned rows = min(s.x.n_tok, p.tile_tok) * p.group_heads;  // as in part_of
+  const unsigned entries = s.pieces <= 1 ? 0 : entries_of(s.blocks, s.pieces, s.few);
   const float want = static_cast<float>(s.tiles) * static_cast<float>(p.groups) *
-                     static_cast<float>(s.blocks) * static_cast<float>(rows);
+                     static_cast<float>(entries) * static_cast<float>(rows);
   s.slots = s.pieces <= 1 ? 0u : want >= static_cast<float>(kMuch) ? kMuch
-                                     : static_cast<unsigned>(s.tiles) * p.groups * s.blocks * rows;
+                                     : static_cast<unsigned>(s.tiles) * p.groups * entries * rows;
 }
 // With `end` the slots up to its own: a request whose results do not fit is not split.
 __device__ __forceinline__ void count_items(const Params& p, unsigned end, Share& s) {
@@ -260,7 +277,7 @@ __device__ __forceinline__ Work work_of(const Params& p, int r, const Request& x
   Work w;
   w.r = r;
   w.pieces = pieces;
-  w.blocks = blocks;
+  w.entries = entries_of(blocks, pieces, is_few(p, x));
   w.base = base;
   w.x = x;
   w.group = divide(in, per_group);
@@ -319,7 +336,10 @@ struct Finder {
     for (int h = 0; h < 2; ++h) {
       if (s[h].few) at[h] += many0;
       const int r = lane + 32 * h;
-      if (publish && r < p.R) p.info[r] = make_int4(s[h].pieces, s[h].blocks, base[h], 0);
+      if (publish && r < p.R) {
+        const int entries = s[h].pieces > 1 ? entries_of(s[h].blocks, s[h].pieces, s[h].few) : 0;
+        p.info[r] = make_int4(s[h].pieces, entries, base[h], 0);
+      }
     }
     if (publish) {
       split = __any_sync(0xffffffffu, split);
@@ -367,8 +387,8 @@ struct Finder {
   }
 };
 
-// Where the partial results of block i of a tile's list are, of which a request keeps `rows` per
-// tile and block: first the place of row 0's (m, l) and of its columns.  Columns lie four by
+// Where partial result i of a tile is, of which a request keeps `entries` per tile and `rows`
+// per entry: first the place of row 0's (m, l) and of its columns.  Columns lie four by
 // four, a row's four next to the other rows', so that a warp with a row per lane stores (and the
 // join, with a few rows per warp, reads) whole sectors: row by row, 64 KiB took a block 9000
 // clocks to leave.
@@ -380,10 +400,10 @@ __device__ __forceinline__ int part_rows(const Params& p, const Request& x) {
   return min(x.n_tok, p.tile_tok) * p.group_heads;
 }
 __device__ __forceinline__ Part part_of(const Params& p, const Request& x, unsigned base,
-                                        int blocks, int tile, int group, int i) {
+                                        int entries, int tile, int group, int i) {
   const int rows = part_rows(p, x);
   return {static_cast<int64_t>(base) +
-              (static_cast<int64_t>(tile * p.groups + group) * blocks + i) * rows,
+              (static_cast<int64_t>(tile * p.groups + group) * entries + i) * rows,
           rows};
 }
 // Column col (a multiple of 4) of `row`.

@@ -237,7 +237,8 @@ __device__ __forceinline__ void weights_of(const uint32_t (&s)[32], uint64_t sca
 struct Item {
   int pieces;             // 0: it is not there
   int r, kvh, tok;        // request, KV head, first row
-  Part part;              // its partial results, of the list's first block (pieces > 1)
+  bool joins;             // keeps a running result of its blocks (else they leave theirs)
+  Part part;              // its first partial result (pieces > 1)
   int n_tok, rows, tok0;  // its tile (tok0 in the request)
   int pos0, pmax;         // positions of its first and last token
   // the keys it walks: blocks [i0, i1) of `list`.  Items that share K and V walk the keys that
@@ -265,6 +266,7 @@ __device__ __forceinline__ void make_items(const Params& p, const Work (&found)[
   const int lane = threadIdx.x & 15, k = (threadIdx.x & 31) >> 4;
   Item it;
   it.pieces = 0;
+  it.joins = true;
   it.r = it.kvh = it.tok = 0;
   it.part = Part{0, 0};
   it.n_tok = it.rows = it.tok0 = it.pos0 = it.i0 = it.i1 = it.steps = 0;
@@ -275,7 +277,6 @@ __device__ __forceinline__ void make_items(const Params& p, const Work (&found)[
     it.pieces = w.pieces;
     it.r = w.r;
     it.kvh = w.kvh;
-    it.part = part_of(p, w.x, w.base, w.blocks, w.tile, w.group, 0);
     it.tok0 = w.tile * p.tile_tok;
     it.tok = w.x.tok + it.tok0;
     it.n_tok = min(p.tile_tok, w.x.n_tok - it.tok0);
@@ -292,6 +293,10 @@ __device__ __forceinline__ void make_items(const Params& p, const Work (&found)[
     it.list = block_list(p, it.list_pos0, it.list_pmax);
     it.i0 = piece_start(it.list.n, w.piece, w.pieces);
     it.i1 = piece_start(it.list.n, w.piece + 1, w.pieces);
+    const bool few = is_few(p, w.x);
+    it.joins = w.pieces == 1 || (!few && w.piece == 0);
+    it.part = part_of(p, w.x, w.base, w.entries, w.tile, w.group,
+                      first_entry(it.list.n, w.piece, w.pieces, few, it.i0));
     for (int i = it.i0 + lane; i < it.i1; i += 16) {
       it.steps += __popc(steps_of(p, it, it.list.at(i)));
     }
@@ -630,11 +635,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       return t0 + kTile - 1 <= pos0 &&
              (p.window == INT32_MAX || t0 > pmax - p.window || t0 + kTile <= p.first);
     };
-    // The finished key block's O, with its (bm, bl): joined to the running result, or (split
-    // items) left for the join.
-    auto close_block = [&](float bm, float bl) {
-      if (pieces > 1) {
-        const Part at = {item.part.first + static_cast<int64_t>(item.i0 + block) * item.part.rows,
+    // Leaves what O holds for the join, with its (bm, bl), as the item's partial result `entry`.
+    auto leave = [&](int entry, float bm, float bl) {
+        const Part at = {item.part.first + static_cast<int64_t>(entry) * item.part.rows,
                          item.part.rows};
         if (live) p.part_ml[at.first + row] = make_float2(bm, bl);
 #pragma unroll 1
@@ -652,6 +655,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
+    };
+    // The finished key block's O, with its (bm, bl): joined to the running result, or (in a
+    // later piece) left for the join.
+    auto close_block = [&](float bm, float bl) {
+      if (!item.joins) {
+        leave(block, bm, bl);
       } else {
         float fa, fb;
         fold_factors(tot_m, bm, fa, fb);
@@ -902,7 +911,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ok && steps > 0) {
       ok = warp_wait(&sh.o_full[k], 0, abort_flag);
       tc_fence_after();
-      if (ok && warp_live) close_block(m, l);
+      if (ok && warp_live) {
+        close_block(m, l);
+        if (item.joins && pieces > 1) {  // the running result, by way of O's columns
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              float x0, x1;
+              unpair(tot_o[(c + j) / 2], x0, x1);
+              o[j] = __float_as_uint(x0);
+              o[j + 1] = __float_as_uint(x1);
+            }
+            tmem_st_x32(tO + c, o);
+          }
+          tmem_st_wait();
+          leave(0, tot_m, tot_l);
+        }
+      }
     }
     if (!ok) {
       if (lane == 0) {
