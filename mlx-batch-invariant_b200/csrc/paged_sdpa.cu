@@ -58,7 +58,10 @@ __global__ void __launch_bounds__(kSimtThreads) paged_simt_kernel(const Params p
     Finder finder;
     finder.begin(p, blockIdx.x == 0);
     const bool there = blockIdx.x < finder.total;
-    if (there) finder.find(p, blockIdx.x, &s_work);
+    if (there) {
+      const Work w = finder.find(p, blockIdx.x, blockIdx.x);
+      if (threadIdx.x == 0) s_work = w;
+    }
     if (threadIdx.x == 0) s_there = there;
   }
   __syncthreads();

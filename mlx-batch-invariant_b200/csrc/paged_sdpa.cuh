@@ -208,11 +208,11 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int d = 16; d > 0; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
   return v;
 }
-// Inclusive scan over a warp (sums above kMuch stay there).
-__device__ __forceinline__ unsigned warp_scan(unsigned a) {
+// Inclusive scan over a warp's first n lanes (sums above kMuch stay there).
+__device__ __forceinline__ unsigned warp_scan(unsigned a, int n = 32) {
   const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int d = 1; d < 32; d *= 2) {
+#pragma unroll 1
+  for (int d = 1; d < n; d *= 2) {
     const unsigned x = __shfl_up_sync(0xffffffffu, a, d);
     if (lane >= d) a = add_sat(a, x);
   }
@@ -288,13 +288,14 @@ __device__ __forceinline__ Work work_of(const Params& p, int r, const Request& x
   return w;
 }
 
-constexpr int kFewRequests = 64;
+// (64, two a lane, took longer: a block's search grew by more than the small kernel takes.)
+constexpr int kFewRequests = 32;
 
-// One warp's view of the items.  Up to 64 requests it works them out by itself, two requests a
+// One warp's view of the items.  Up to 32 requests it works them out by itself, a request a
 // lane; beyond, schedule_kernel has left them in the workspace.
 struct Finder {
-  Share s[2];
-  unsigned base[2], at[2];
+  Share s;
+  unsigned base = 0, at = 0;  // its first slot of partial results and first item
   unsigned total;
 
   __device__ __forceinline__ void begin(const Params& p, bool publish) {
@@ -303,87 +304,74 @@ struct Finder {
       total = h.x + h.y;
       return;
     }
-    const int lane = threadIdx.x & 31;
-    s[0] = share_of(p, lane);
-    s[1] = share_of(p, p.R);  // none
-    float load = load_of(s[0]);
-    if (p.R > 32) {
-      s[1] = share_of(p, lane + 32);
-      load += load_of(s[1]);
+    const int lane = threadIdx.x & 31, n = p.R;
+    s = share_of(p, lane);
+    split_share(p, spans_of(p, warp_sum(load_of(s))), s);
+    unsigned end = 0, many = 0, few = 0;
+    if (__any_sync(0xffffffffu, s.slots != 0)) end = warp_scan(s.slots, n);
+    base = end - s.slots;
+    count_items(p, end, s);
+    if (__any_sync(0xffffffffu, !s.few && s.items != 0)) {
+      many = warp_scan(s.few ? 0 : s.items, n);
+      at = many - s.items;
+      many = __shfl_sync(0xffffffffu, many, n - 1);
     }
-    const Spans sp = spans_of(p, warp_sum(load));
-    unsigned slots0 = 0, many0 = 0, few0 = 0, split = 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      base[h] = at[h] = 0;
-      s[h].items = s[h].pieces = 0;
-      if (h == 1 && p.R <= 32) continue;
-      split_share(p, sp, s[h]);
-      unsigned end = slots0;
-      if (__any_sync(0xffffffffu, s[h].slots != 0)) end = add_sat(slots0, warp_scan(s[h].slots));
-      base[h] = end - s[h].slots;
-      slots0 = __shfl_sync(0xffffffffu, end, 31);
-      count_items(p, end, s[h]);
-      split |= s[h].pieces > 1;
-      const unsigned m = warp_scan(s[h].few ? 0 : s[h].items);
-      const unsigned f = warp_scan(s[h].few ? s[h].items : 0);
-      at[h] = (s[h].few ? few0 + f : many0 + m) - s[h].items;
-      many0 += __shfl_sync(0xffffffffu, m, 31);
-      few0 += __shfl_sync(0xffffffffu, f, 31);
+    if (__any_sync(0xffffffffu, s.few && s.items != 0)) {
+      few = warp_scan(s.few ? s.items : 0, n);
+      if (s.few) at = many + few - s.items;
+      few = __shfl_sync(0xffffffffu, few, n - 1);
     }
-    total = many0 + few0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (s[h].few) at[h] += many0;
-      const int r = lane + 32 * h;
-      if (publish && r < p.R) {
-        const int entries = s[h].pieces > 1 ? entries_of(s[h].blocks, s[h].pieces, s[h].few) : 0;
-        p.info[r] = make_int4(s[h].pieces, entries, base[h], 0);
-      }
-    }
+    total = many + few;
     if (publish) {
-      split = __any_sync(0xffffffffu, split);
-      if (lane == 0) *p.head = make_int4(many0, few0, split, 0);
+      if (lane < n) {
+        const int entries = s.pieces > 1 ? entries_of(s.blocks, s.pieces, s.few) : 0;
+        p.info[lane] = make_int4(s.pieces, entries, base, 0);
+      }
+      const unsigned split = __any_sync(0xffffffffu, s.pieces > 1);
+      if (lane == 0) *p.head = make_int4(many, few, split, 0);
     }
   }
 
-  // Item i < total, to `out` (shared memory), by the whole warp.
-  __device__ __forceinline__ void find(const Params& p, unsigned i, Work* out) const {
+  // Items i0 < total and i1 < total, by the whole warp: lanes 0..15 get item i0, the others i1.
+  __device__ __forceinline__ Work find(const Params& p, unsigned i0, unsigned i1) const {
     const int lane = threadIdx.x & 31;
+    const unsigned i = lane < 16 ? i0 : i1;
     if (p.R <= kFewRequests) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const Share& x = s[h];
-        if (i >= at[h] && i < at[h] + x.items) {
-          *out = work_of(p, lane + 32 * h, x.x, x.tiles, x.blocks, x.pieces, base[h], i - at[h]);
-        }
-      }
-      return;
+      const unsigned has0 = __ballot_sync(0xffffffffu, i0 - at < s.items);
+      const unsigned has1 = __ballot_sync(0xffffffffu, i1 - at < s.items);
+      const int r = __ffs(lane < 16 ? has0 : has1) - 1;
+      auto pick = [&](unsigned a) { return __shfl_sync(0xffffffffu, a, r); };
+      Request x;
+      x.tok = pick(s.x.tok);
+      x.n_tok = pick(s.x.n_tok);
+      x.seq = pick(s.x.seq);
+      const int tiles = pick(s.tiles), blocks = pick(s.blocks);
+      const unsigned pieces = pick(s.pieces), b = pick(base), first = pick(at);
+      return work_of(p, r, x, tiles, blocks, pieces, b, i - first);
     }
-    // the first request whose end lies behind the item, 32-way
+    // the first request whose end lies behind the item, 16-way
     const unsigned many = p.head->x;
     const bool few = i >= many;
     const unsigned v = few ? i - many : i;
+    const int half = lane & 16, in = lane & 15;
     int lo = 0, n = p.R;  // it is among [lo, lo + n)
-    while (n > 1) {
-      const int step = (n + 31) / 32;
-      const int last = min(lo + (lane + 1) * step, lo + n) - 1;  // of this lane's part
+    while (__any_sync(0xffffffffu, n > 1)) {
+      const int step = (n + 15) / 16;
+      const int last = min(lo + (in + 1) * step, lo + n) - 1;  // of this lane's part
       const int2 e = p.ends[last];
       const unsigned behind =
-          __ballot_sync(0xffffffffu, static_cast<unsigned>(few ? e.y : e.x) > v);
+          __ballot_sync(0xffffffffu, static_cast<unsigned>(few ? e.y : e.x) > v) >> half & 0xffffu;
       const int k = __ffs(behind) - 1;  // (there is one: i < total)
       const int start = lo + k * step;
       n = min(step, lo + n - start);
       lo = start;
     }
-    if (lane == 0) {
-      const Share x = share_of(p, lo);
-      const int4 info = p.info[lo];
-      const unsigned items = x.tiles * info.x * p.groups;
-      const int2 e = p.ends[lo];
-      *out = work_of(p, lo, x.x, x.tiles, x.blocks, info.x, info.z,
-                     v - (static_cast<unsigned>(few ? e.y : e.x) - items));
-    }
+    const Share x = share_of(p, lo);
+    const int4 info = p.info[lo];
+    const unsigned items = x.tiles * info.x * p.groups;
+    const int2 e = p.ends[lo];
+    return work_of(p, lo, x.x, x.tiles, x.blocks, info.x, info.z,
+                   v - (static_cast<unsigned>(few ? e.y : e.x) - items));
   }
 };
 

@@ -260,10 +260,16 @@ __device__ __forceinline__ unsigned steps_of(const Params& p, const Item& it, in
   return set;
 }
 
-// Describes the block's items (of which `there` exist), 16 lanes of a warp each.
-__device__ __forceinline__ void make_items(const Params& p, const Work (&found)[2], int there,
-                                           bool shared, Item (&out)[2]) {
+// Describes the block's items (of which `there` exist): lanes 0..15 of a warp have the first
+// one's `w`, the others the second's.  Says whether they share K and V: two tiles of one request
+// and group, whose keys are not split.
+__device__ __forceinline__ bool make_items(const Params& p, const Work& w, int there,
+                                           Item (&out)[2]) {
   const int lane = threadIdx.x & 15, k = (threadIdx.x & 31) >> 4;
+  const int other = __shfl_xor_sync(0xffffffffu, w.tile, 16);
+  const bool same = __shfl_xor_sync(0xffffffffu, w.r, 16) == w.r &&
+                    __shfl_xor_sync(0xffffffffu, w.group, 16) == w.group;
+  const bool shared = there == 2 && same && w.pieces == 1;
   Item it;
   it.pieces = 0;
   it.joins = true;
@@ -273,7 +279,6 @@ __device__ __forceinline__ void make_items(const Params& p, const Work (&found)[
   it.pmax = it.list_pos0 = it.list_pmax = -1;
   it.list = BlockList{0, 0, 0, 0};
   if (k < there) {
-    const Work& w = found[k];
     it.pieces = w.pieces;
     it.r = w.r;
     it.kvh = w.kvh;
@@ -287,8 +292,8 @@ __device__ __forceinline__ void make_items(const Params& p, const Work (&found)[
     it.list_pos0 = it.pos0;
     it.list_pmax = it.pmax;
     if (shared) {  // item 1 is the tile before item 0's
-      it.list_pos0 = first + found[1].tile * p.tile_tok;
-      it.list_pmax = first + min((found[0].tile + 1) * p.tile_tok, w.x.n_tok) - 1;
+      it.list_pos0 = first + min(w.tile, other) * p.tile_tok;
+      it.list_pmax = first + min((max(w.tile, other) + 1) * p.tile_tok, w.x.n_tok) - 1;
     }
     it.list = block_list(p, it.list_pos0, it.list_pmax);
     it.i0 = piece_start(it.list.n, w.piece, w.pieces);
@@ -305,6 +310,7 @@ __device__ __forceinline__ void make_items(const Params& p, const Work (&found)[
 #pragma unroll
   for (int d = 8; d > 0; d /= 2) it.steps += __shfl_xor_sync(0xffffffffu, it.steps, d);
   if (lane == 0) out[k] = it;
+  return shared;
 }
 
 // Walks an item's steps.
@@ -337,7 +343,6 @@ __device__ __forceinline__ int v_place(bool shared, int l0, int l1, int k, int j
 }
 
 struct Shared {
-  Work found[2];
   uint64_t q_full[2], full[kMaxStages], empty[kMaxStages], s_full[2], p_half[2], p_ready[2],
       o_full[2], mma_done;
   uint32_t tmem;
@@ -395,19 +400,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const unsigned per = 2 * finder.total <= static_cast<unsigned>(p.target) ? 1 : 2;
     const unsigned at = blockIdx.x * per;
     const int there = at >= finder.total ? 0 : min(per, finder.total - at);
-#pragma unroll 1
-    for (int k = 0; k < there; ++k) finder.find(p, at + k, &sh.found[k]);
-    __syncwarp();
-    // two tiles of one request and group, their keys not split: they share K and V
-    const bool both = there == 2 && sh.found[0].r == sh.found[1].r &&
-                      sh.found[0].group == sh.found[1].group && sh.found[0].pieces == 1;
-    make_items(p, sh.found, there, both, sh.item);
+    Work w = {};
+    if (there > 0) w = finder.find(p, at, at + there - 1);
+    const bool both = make_items(p, w, there, sh.item);
     if (lane == 0) sh.shared = both;
-  }
-  __syncthreads();
-  if (sh.item[0].pieces == 0) return;
-  const bool shared = sh.shared;
-  if (warp == 9) {
+  } else if (warp == 9) {
     tmem_alloc(&sh.tmem, kTmemCols);
     tmem_relinquish();
   }
@@ -416,7 +413,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-
+  if (sh.item[0].pieces == 0) {
+    if (warp == 9) tmem_dealloc(tmem, kTmemCols);
+    return;
+  }
+  const bool shared = sh.shared;
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == 8) {
