@@ -210,6 +210,21 @@ SMALL_DECODER = dict(layers=2, hidden=1024, heads=16, kv_heads=8, head_dim=64, i
                      vocab=4096)
 
 
+def _paged_check(dec, model, args, dev):
+    """Over a paged cache: request 0's logits served alone and in one piece against those in
+    the full batch with every prompt in chunks.  (steps that differ, steps)"""
+    ids = dec.prompts(model.cfg, args.batch, args.prompt, dev)
+    per = (args.prompt + args.gen + args.page - 1) // args.page
+    out = []
+    for B, chunk in ((1, None), (args.batch, max(1, args.prompt // 3))):
+        server = dec.PagedDecoder(model, B, B * per, args.page)
+        graph = dec.PagedDecodeGraph(server) if args.gen and not args.eager else None
+        out.append(dec.generate_paged(server, ids[:B], args.gen, chunk, graph)[0])
+        del graph
+    d = dec.differing(dec.slot0_bits(out[1][:, None]), dec.slot0_bits(out[0][:, None]))
+    return sum(1 for n in d if n), len(d)
+
+
 def decoder(argv=None):
     """The end-to-end check of the reference's bench/bench.py:211-246 (determinism) and
     :161-208 (e2e) on the Llama-shaped decoder: the slot-0 logits of every prefill and
@@ -233,6 +248,10 @@ def decoder(argv=None):
                    help="decode step by step from Python instead of replaying a CUDA graph")
     p.add_argument("--single-check", action="store_true",
                    help="under torchrun: also run the unsharded model on every rank")
+    p.add_argument("--paged", action="store_true",
+                   help="also serve the prompts over a KV cache in pages, in chunks and mixed "
+                        "with decoding requests")
+    p.add_argument("--page", type=int, default=64, help="tokens of a page (--paged)")
     p.add_argument("--json", help="write the results here (rank 0)")
     args = p.parse_args(argv)
 
@@ -292,6 +311,12 @@ def decoder(argv=None):
                                                         len(diff) * cfg.vocab))
     results["invariant"] = {"batch": args.batch, "steps_differing": bad, "steps": len(diff),
                             "logits_differing": sum(diff)}
+    if args.paged:
+        with batch_invariant_mode(strict=True):
+            bad, steps = _paged_check(dec, model, args, dev)
+        fails += bad > 0
+        say("| in pages of %d, chunked | %d | %d / %d | |" % (args.page, args.batch, bad, steps))
+        results["paged"] = {"page": args.page, "steps_differing": bad, "steps": steps}
     if world == 1 and not args.no_stock:
         stock = {}
         for B in sorted({1, args.batch}):
@@ -342,7 +367,7 @@ def main(argv=None):
         return decoder(argv[1:])
     print("usage: mlx-bi verify [--quick] [--dtype float32|float16|bfloat16] [--seed N]\n"
           "       mlx-bi decoder [--small] [--batch B] [--prompt L] [--gen S] "
-          "[--exchange fused|nccl] [--single-check]\n"
+          "[--exchange fused|nccl] [--single-check] [--paged [--page P]]\n"
           "(or python -m mlx_batch_invariant_b200 ...)", file=sys.stderr)
     return 2
 

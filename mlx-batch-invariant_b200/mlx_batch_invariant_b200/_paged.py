@@ -76,8 +76,8 @@ def paged_plan(query_lens, context_lens, block_table, page_size, num_tokens, *, 
     """
     compiling = torch.compiler.is_compiling()
     if not compiling:
-        out = (_lib._short or _lib.short_way()).plan(query_lens, context_lens, block_table, page_size, num_tokens,
-                            free_pages, free_head)
+        out = (_lib._short or _lib.short_way()).plan(
+            query_lens, context_lens, block_table, page_size, num_tokens, free_pages, free_head)
         if out.__class__ is tuple:
             return _new_tuple(PagedPlan, out)
         if out is not None:
@@ -179,7 +179,8 @@ def rope_kv_paged(qkv, cos, sin, positions, slots, k_cache, v_cache, *, out=None
     """
     compiling = torch.compiler.is_compiling()
     if not compiling:
-        q = (_lib._short or _lib.short_way()).rope(qkv, cos, sin, positions, slots, k_cache, v_cache, out)
+        q = (_lib._short or _lib.short_way()).rope(qkv, cos, sin, positions, slots, k_cache,
+                                                   v_cache, out)
         if q.__class__ is not int and q is not None:
             return q
         if q is not None:
@@ -252,8 +253,9 @@ def paged_attention(q, k_cache, v_cache, block_table, query_start, seq_lens, *, 
     """
     compiling = torch.compiler.is_compiling()
     if not compiling:
-        o = (_lib._short or _lib.short_way()).attention(q, k_cache, v_cache, block_table, query_start, seq_lens, scale,
-                               window, first_tokens, sinks, out)
+        o = (_lib._short or _lib.short_way()).attention(
+            q, k_cache, v_cache, block_table, query_start, seq_lens, scale, window, first_tokens,
+            sinks, out)
         if o.__class__ is not int and o is not None:
             return o
         if o is not None:

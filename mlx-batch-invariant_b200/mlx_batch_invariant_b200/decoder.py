@@ -26,6 +26,11 @@ replicated rows; RoPE with the KV-cache write, and SwiGLU, are two fused libbi.s
 kernels (bi_rope_kv, bi_swiglu) on CUDA and the equivalent torch expressions on CPU.
 Each computes every output element on its own, so all are batch-invariant on B200
 (tests/test_mode_gpu.py and tests/test_decoder_gpu.py guard that).
+
+PagedDecoder serves the same weights over a KV cache in pages: requests of any length
+side by side, prompts in chunks of any size next to decoding requests, pages taken from
+and given back to a free list (paged_plan, rope_kv_paged, paged_attention).  A request's
+logits are bitwise those it gets alone (tests/test_paged_decoder_gpu.py).
 """
 
 import dataclasses
@@ -38,6 +43,7 @@ import torch.nn.functional as F
 
 from . import _lib, parallel
 from ._attention import scaled_dot_product_attention
+from ._paged import paged_attention, paged_plan, rope_kv_paged
 
 
 @dataclasses.dataclass(frozen=True)
@@ -215,6 +221,22 @@ class Decoder:
             raise NotImplementedError("the stock path prefills from position 0 only")
         return F.scaled_dot_product_attention(q, k, v, is_causal=L > 1, enable_gqa=True)
 
+    def _behind_attention(self, x, a, p):
+        """The rest of a layer: x and the attention's heads a (..., hq * hd) of this rank."""
+        cfg = self.cfg
+        d = cfg.hidden
+        a = self._gather(a, cfg.heads * cfg.head_dim)
+        x = x + self._column(a, p["wo"], d, d)
+        y = F.rms_norm(x, (d,), p["n2"], cfg.eps)
+        gu = F.linear(y, p["wgu"])
+        if self.device.type == "cuda":
+            act = self._swiglu(gu)
+        else:
+            gate, up = gu.split((self.inter_local, self.inter_local), dim=-1)
+            act = F.silu(gate) * up
+        act = self._gather(act, cfg.inter)
+        return x + self._column(act, p["wd"], d, d)
+
     # ------------------------------------------------------------------ forward
     def _forward(self, ids, pos=None):
         """Logits of each row's last position.  pos None: the host position self.pos
@@ -261,17 +283,7 @@ class Decoder:
                 a = self._attention(q, ck, cv, 1, mask)
             else:
                 a = self._attention(q, ck[:, :, :p0 + L], cv[:, :, :p0 + L], L)
-            a = self._gather(a.transpose(1, 2).reshape(B, L, hq * hd), cfg.heads * hd)
-            x = x + self._column(a, p["wo"], d, d)
-            y = F.rms_norm(x, (d,), p["n2"], cfg.eps)
-            gu = F.linear(y, p["wgu"])
-            if native:
-                act = self._swiglu(gu)
-            else:
-                gate, up = gu.split((self.inter_local, self.inter_local), dim=-1)
-                act = F.silu(gate) * up
-            act = self._gather(act, cfg.inter)
-            x = x + self._column(act, p["wd"], d, d)
+            x = self._behind_attention(x, a.transpose(1, 2).reshape(B, L, hq * hd), p)
         if not static:
             self.pos += L
         h = F.rms_norm(x[:, -1], (d,), self.norm, cfg.eps)
@@ -342,6 +354,192 @@ class DecodeGraph:
         self.graph.replay()
         self._next = nxt + 1
         return self.logits
+
+
+class PagedDecoder:
+    """A Decoder's weights serving up to `requests` sequences over a KV cache in `pages` pages
+    of `page_size` tokens per layer.
+
+    step() runs the new tokens of any of the requests -- a prompt, a chunk of one, a decoded
+    token -- together; release() ends a sequence and gives its pages back.  Each request's
+    logits are bitwise those it gets alone and with its prompt in one piece.  The host knows
+    every length, so what does not fit is refused before anything is enqueued.
+    """
+
+    def __init__(self, model, requests, pages, page_size=64):
+        if model.device.type != "cuda":
+            raise ValueError("the paged cache takes a model on a CUDA device, got %s"
+                             % model.device)
+        if requests < 1 or pages < 1 or page_size < 1:
+            raise ValueError("requests, pages and page_size must be positive")
+        if model._fused and requests > model.max_batch:
+            raise ValueError("%d requests exceed the exchange buffers' %d"
+                             % (requests, model.max_batch))
+        self.model, self.page_size = model, page_size
+        self.requests, self.pages = requests, pages
+        dev = model.device
+        shape = (pages, model.hk, page_size, model.cfg.head_dim)
+        self.cache_k = [torch.zeros(shape, dtype=model.dtype, device=dev) for _ in model.layers]
+        self.cache_v = [torch.zeros(shape, dtype=model.dtype, device=dev) for _ in model.layers]
+        width = (model.max_len + page_size - 1) // page_size
+        self.table = torch.full((requests, width), -1, dtype=torch.int32, device=dev)
+        self.free_pages = torch.arange(pages, dtype=torch.int32, device=dev)
+        self.free_head = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.context_lens = torch.zeros(requests, dtype=torch.int32, device=dev)
+        self.lens = [0] * requests  # the same on the host
+        self._rows = torch.arange(requests, device=dev)
+
+    def _pages_of(self, tokens):
+        return (tokens + self.page_size - 1) // self.page_size
+
+    @property
+    def pages_used(self):
+        return sum(self._pages_of(n) for n in self.lens)
+
+    def _lens_after(self, query_lens):
+        """The requests' lengths behind a step of query_lens new tokens, which must fit."""
+        new = [n + q for n, q in zip(self.lens, query_lens)]
+        for r, n in enumerate(new):
+            if n > self.model.max_len:
+                raise ValueError("request %d would have %d tokens, the cache holds %d"
+                                 % (r, n, self.model.max_len))
+        need = sum(self._pages_of(n) for n in new)
+        if need > self.pages:
+            raise ValueError("the step needs %d pages, the cache has %d" % (need, self.pages))
+        most = self.model.max_batch * self.model.max_len
+        if self.model._fused and sum(query_lens) > most:
+            raise ValueError("%d tokens exceed the exchange buffers' %d"
+                             % (sum(query_lens), most))
+        return new
+
+    def _run(self, ids, query_lens):
+        """Device work of a step: ids (T,) in request order, query_lens (requests,) int32."""
+        m, cfg = self.model, self.model.cfg
+        d, hd = cfg.hidden, cfg.head_dim
+        T = ids.shape[0]
+        plan = paged_plan(query_lens, self.context_lens, self.table, self.page_size, T,
+                          free_pages=self.free_pages, free_head=self.free_head)
+        x = F.embedding(ids, m.embed)
+        for p, ck, cv in zip(m.layers, self.cache_k, self.cache_v):
+            qkv = F.linear(F.rms_norm(x, (d,), p["n1"], cfg.eps), p["wqkv"])
+            q = rope_kv_paged(qkv, m.cos, m.sin, plan.positions, plan.slots, ck, cv)
+            a = paged_attention(q, ck, cv, self.table, plan.query_start, plan.seq_lens,
+                                scale=1.0 / math.sqrt(hd))
+            x = m._behind_attention(x, a.reshape(T, m.hq * hd), p)
+        self.free_head.copy_(plan.next_head)
+        self.context_lens.copy_(plan.seq_lens)
+        last = (plan.query_start[1:] - 1).clamp(min=0).long()
+        h = F.rms_norm(x.index_select(0, last), (d,), m.norm, cfg.eps)
+        return m._column(h, m.head, cfg.vocab, "head")
+
+    def step(self, new_tokens):
+        """new_tokens: per request a sequence of token ids (empty or None: none).  Logits
+        (requests, vocab) of each request's last token; rows of requests without new tokens
+        hold no answer."""
+        if len(new_tokens) != self.requests:
+            raise ValueError("%d entries for %d requests" % (len(new_tokens), self.requests))
+        new = [[] if t is None else t.tolist() if isinstance(t, torch.Tensor) else list(t)
+               for t in new_tokens]
+        query_lens = [len(t) for t in new]
+        if not any(query_lens):
+            raise ValueError("the step has no tokens")
+        for t in new:
+            if t and not 0 <= min(t) <= max(t) < self.model.cfg.vocab:
+                raise ValueError("token ids must be in [0, %d)" % self.model.cfg.vocab)
+        lens, dev = self._lens_after(query_lens), self.model.device
+        ids = torch.tensor([x for t in new for x in t], dtype=torch.long).to(dev)
+        logits = self._run(ids, torch.tensor(query_lens, dtype=torch.int32).to(dev))
+        self.lens = lens
+        return logits
+
+    def release(self, request):
+        """Ends a request's sequence: its pages go back to the list."""
+        n, used = self._pages_of(self.lens[request]), self.pages_used
+        self.free_pages[used - n:used] = self.table[request, :n]
+        self.free_head.fill_(used - n)
+        self.context_lens[request] = 0
+        self.lens[request] = 0
+
+
+class PagedDecodeGraph:
+    """One greedy decode step of a PagedDecoder's running requests, captured once in a CUDA
+    graph: the tokens, the lengths and which requests run live on the device, so a replay
+    serves any set of them at any lengths.  Capture inside batch_invariant_mode."""
+
+    def __init__(self, server):
+        self.server = server
+        dev, R = server.model.device, server.requests
+        self.tok = torch.zeros(R, dtype=torch.long, device=dev)
+        self.running = torch.zeros(R, dtype=torch.int32, device=dev)  # (none: a step of padding)
+        self._active = [0] * R
+        side = torch.cuda.Stream(device=dev)
+        side.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(side):
+            self._greedy()
+        torch.cuda.current_stream(dev).wait_stream(side)
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph):
+            self.logits = self._greedy()
+
+    def _greedy(self):
+        # row i belongs to the (i + 1)-th running request
+        ends = torch.cumsum(self.running, 0)
+        row = torch.searchsorted(ends, self.server._rows, right=True)
+        ids = self.tok[row.clamp(max=self.server.requests - 1)]
+        logits = self.server._run(ids, self.running)
+        self.tok.copy_(torch.where(self.running > 0, logits.argmax(dim=-1), self.tok))
+        return logits
+
+    def start(self, tokens):
+        """tokens: per request the token to go on from, or None for one that does not run."""
+        if len(tokens) != self.server.requests:
+            raise ValueError("%d entries for %d requests" % (len(tokens), self.server.requests))
+        self._active = [int(t is not None) for t in tokens]
+        self.tok.copy_(torch.tensor([0 if t is None else int(t) for t in tokens]))
+        self.running.copy_(torch.tensor(self._active, dtype=torch.int32))
+
+    def step(self):
+        """One decode step; returns the graph's logits buffer (overwritten by the next)."""
+        if not any(self._active):
+            raise RuntimeError("PagedDecodeGraph.start() must name a running request first")
+        lens = self.server._lens_after(self._active)
+        self.graph.replay()
+        self.server.lens = lens
+        return self.logits
+
+
+def generate_paged(server, ids, steps, chunk=None, graph=None):
+    """Greedy over pages: the prompts ids (B, L) in chunks of `chunk` tokens (None: whole),
+    each request's chunks beginning one step after the request before it, so that prompts
+    share steps with requests that decode already; then on to `steps` decoded tokens for
+    each.  `graph`, a PagedDecodeGraph, takes the steps in which every request decodes.
+    Returns per request its (steps + 1, vocab) logits."""
+    B, L = ids.shape
+    chunk = L if chunk is None else chunk
+    prompt = ids.tolist()
+    out = [[] for _ in range(B)]
+    todo = [None] * B  # the decoding requests' next tokens
+    at = 0
+    while any(len(o) <= steps for o in out):
+        new = [None] * server.requests
+        for b in range(B):
+            if len(out[b]) > steps or at < b:
+                continue
+            lo = (at - b) * chunk
+            new[b] = prompt[b][lo:lo + chunk] if lo < L else [todo[b]]
+        at += 1
+        decoding = [b for b in range(B) if new[b] is not None and out[b]]
+        if graph is not None and decoding and len(decoding) == sum(n is not None for n in new):
+            graph.start([None if n is None else n[0] for n in new])
+            logits = graph.step().clone()
+        else:
+            logits = server.step(new)
+        best = logits.argmax(dim=-1).tolist()
+        for b in range(B):
+            if new[b] is not None and server.lens[b] >= L:
+                out[b].append(logits[b])
+                todo[b] = best[b]
+    return [torch.stack(o) for o in out]
 
 
 def generate(model, ids, steps, graph=None):
