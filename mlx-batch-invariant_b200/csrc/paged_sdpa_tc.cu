@@ -14,7 +14,20 @@
 // One thread issues both items' products in turn, so while one item's products run the other's
 // softmax does: two blocks per SM with an item each fell into step, both in their softmax at
 // one time and both waiting for the tensor pipe at another (5000 clocks for two tiles of 128
-// keys where the products take 2048).
+// keys where the products take 2048; now 3900).
+//
+// Bound, for chunks, by the chain of a step, which two items overlap only in part and TMEM has
+// no room for a third: scores 300 clocks behind the product, maximum 500, exponentials 1900
+// (the special-function unit alone takes 1024), the product's turn 1100.  2048 tokens behind
+// 6144, 32 heads of 128 over 8: 280 us, 860 TFLOP/s, 51 % of cuBLAS's burst rate; tensor pipe
+// 38 %, special-function unit 47 %, issue slots 36 % of the time.  For decode by HBM and, of a
+// block's 50 us, the 5 until its first product: 64 requests of 3000 to 8191 keys take 273 us,
+// 5.3 TB/s, 82 % of the copy rate.
+//
+// P is rounded to the caches' 16-bit type because a product's two operands have one type and V
+// has that one; the row's sum adds the weights before that rounding.  It adds half a step of the
+// type (2^-9 for bf16, 2^-12 for fp16) to each weight, independent from key to key: the result
+// is off by 0.0023 of its norm in bf16, where rounding the exact one is off by 0.0017.
 //
 // The running maximum of a 512-key block only moves when a tile's exceeds it by more than
 // 2^8: until then the weights are up to 256 times too large, which the 16-bit type and the
@@ -638,24 +651,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     // Leaves what O holds for the join, with its (bm, bl), as the item's partial result `entry`.
     auto leave = [&](int entry, float bm, float bl) {
-        const Part at = {item.part.first + static_cast<int64_t>(entry) * item.part.rows,
-                         item.part.rows};
-        if (live) p.part_ml[at.first + row] = make_float2(bm, bl);
+      const Part at = {item.part.first + static_cast<int64_t>(entry) * item.part.rows,
+                       item.part.rows};
+      if (live) p.part_ml[at.first + row] = make_float2(bm, bl);
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tmem_ld_32x32b_x32(tO + c, o);
-          tmem_ld_wait(o);
-          if (live) {
-            float4* dst = part_at<D>(p, at, row, c);
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        tmem_ld_32x32b_x32(tO + c, o);
+        tmem_ld_wait(o);
+        if (live) {
+          float4* dst = part_at<D>(p, at, row, c);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              dst[static_cast<int64_t>(j) * at.rows] =
-                  make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]),
-                              __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
-            }
+          for (int j = 0; j < 8; ++j) {
+            dst[static_cast<int64_t>(j) * at.rows] =
+                make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]),
+                            __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
           }
         }
+      }
     };
     // The finished key block's O, with its (bm, bl): joined to the running result, or (in a
     // later piece) left for the join.
