@@ -26,7 +26,7 @@
 //
 // P is rounded to the caches' 16-bit type because a product's two operands have one type and V
 // has that one; the row's sum adds the weights before that rounding.  It adds half a step of the
-// type (2^-9 for bf16, 2^-12 for fp16) to each weight, independent from key to key: the result
+// type (2^-8 for bf16, 2^-11 for fp16) to each weight, independent from key to key: the result
 // is off by 0.0023 of its norm in bf16, where rounding the exact one is off by 0.0017.
 //
 // The running maximum of a 512-key block only moves when a tile's exceeds it by more than
