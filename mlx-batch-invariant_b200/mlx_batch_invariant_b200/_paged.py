@@ -247,7 +247,8 @@ def paged_attention(q, k_cache, v_cache, block_table, query_start, seq_lens, *, 
     ``first_tokens`` first ones.  ``sinks`` is an optional logit per query head, as in
     scaled_dot_product_attention.  Heads are grouped: heads % kv_heads == 0.
 
-    Rows outside every request are not written: pass ``out`` where that matters.  A row that
+    Rows outside every request are not written: pass ``out`` (which may be ``q``) where that
+    matters.  A row that
     sees nothing returns zeros.  Lengths are device data; they are clamped to ``q`` and to the
     table, and pages outside the cache read as zeros.
     """

@@ -516,6 +516,9 @@ def generate_paged(server, ids, steps, chunk=None, graph=None):
     Returns per request its (steps + 1, vocab) logits."""
     B, L = ids.shape
     chunk = L if chunk is None else chunk
+    if B > server.requests or L < 1 or chunk < 1 or steps < 0:
+        raise ValueError("%d prompts of %d tokens in chunks of %d, then %d steps, for %d requests"
+                         % (B, L, chunk, steps, server.requests))
     prompt = ids.tolist()
     out = [[] for _ in range(B)]
     todo = [None] * B  # the decoding requests' next tokens

@@ -45,3 +45,12 @@ def test_pages_are_counted():
         s._lens_after([0, 0, 17, 0])
     with pytest.raises(ValueError, match="exchange"):
         server([0, 0], 99, fused=True)._lens_after([11, 10])
+
+
+def test_what_generate_paged_refuses():
+    s = types.SimpleNamespace(requests=2)
+    ids = torch.zeros((2, 5), dtype=torch.long)
+    for args in ((torch.zeros((3, 5), dtype=torch.long), 1), (ids[:, :0], 1), (ids, 1, 0),
+                 (ids, -1)):
+        with pytest.raises(ValueError, match="prompts"):
+            dec.generate_paged(s, *args)
