@@ -248,9 +248,8 @@ def paged_attention(q, k_cache, v_cache, block_table, query_start, seq_lens, *, 
     scaled_dot_product_attention.  Heads are grouped: heads % kv_heads == 0.
 
     Rows outside every request are not written: pass ``out`` (which may be ``q``) where that
-    matters.  A row that
-    sees nothing returns zeros.  Lengths are device data; they are clamped to ``q`` and to the
-    table, and pages outside the cache read as zeros.
+    matters.  A row that sees nothing returns zeros.  Lengths are device data; they are clamped
+    to ``q`` and to the table, and pages outside the cache read as zeros.
     """
     compiling = torch.compiler.is_compiling()
     if not compiling:
