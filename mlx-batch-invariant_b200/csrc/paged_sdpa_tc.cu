@@ -158,19 +158,6 @@ __device__ __forceinline__ bool elect_one() {
   return yes != 0;
 }
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
-// A vote of an item's four softmax warps; and a barrier of both items'.
-__device__ __forceinline__ bool item_any(int item, bool vote) {
-  uint32_t any;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\t"
-      "bar.red.or.pred q, %1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(any)
-      : "r"(1 + item), "r"(static_cast<uint32_t>(vote))
-      : "memory");
-  return any != 0;
-}
-__device__ __forceinline__ void both_sync() { asm volatile("bar.sync 3, 256;" ::: "memory"); }
-
 // Two fp32 numbers in one 64-bit register, two operations in one instruction, each rounded to
 // nearest.  (Constants are kept packed: a register short, the compiler would otherwise pack
 // them anew at every use.)
@@ -358,12 +345,13 @@ __device__ __forceinline__ int v_place(bool shared, int l0, int l1, int k, int j
 
 struct Shared {
   uint64_t q_full[2], full[kMaxStages], empty[kMaxStages], s_full[2], p_half[2], p_ready[2],
-      o_full[2], mma_done;
+      o_full[2], looked[2], both, mma_done;
   uint32_t tmem;
   int abort_flag;
   int shared;             // the items share K and V
   Item item[2];
   int add[2];             // the item's next product is added to O (it does not start a key block)
+  int hit[2];             // 1 + the last step whose V has such a value
   unsigned bad[2][4];     // keys of a step with a non-finite value that some row sees
 };
 
@@ -396,11 +384,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sh.p_half[k], 4);
       mbar_init(&sh.p_ready[k], 4);
       mbar_init(&sh.o_full[k], 1);
+      mbar_init(&sh.looked[k], 4);
+      sh.hit[k] = 0;
     }
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&sh.full[s], 1);
       mbar_init(&sh.empty[s], 1);
     }
+    mbar_init(&sh.both, 8);
     mbar_init(&sh.mma_done, 1);
     sh.abort_flag = 0;
     fence_barrier_init();
@@ -644,6 +635,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     float m = -INFINITY, l = 0.f;
     bool fresh = true, ok = true;  // fresh: the step starts a key block
     int block = 0;
+    // Barriers of the item's four warps, and of both items' eight, with a bounded wait like all
+    // others (a named barrier would wait for good for a warp that gave up).
+    int n_looked = 0, n_both = 0;
+    auto meet = [&](uint64_t* bar, int& n) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+      return warp_wait(bar, n++ & 1, abort_flag);
+    };
     StepIter it{item.i0, 0, 0};
     // do all rows see every key of the step at t0?
     auto whole_for = [&](int t0, int pos0, int pmax) {
@@ -823,10 +822,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         const bool found = (hit & 0x80008000u) != 0;
-        const bool any = item_any(k, found);  // (both items' warps come to the same answer)
-        if (__builtin_expect(any, 0)) {
+        if (found) *const_cast<volatile int*>(&sh.hit[k]) = step + 1;
+        ok = meet(&sh.looked[k], n_looked);
+        if (!ok) break;
+        // (both items' warps come to the same answer on shared tiles)
+        if (__builtin_expect(*const_cast<volatile int*>(&sh.hit[k]) == step + 1, 0)) {
           // Take them out, and add those that some rows see to these rows' results by hand.
-          if (shared) both_sync();  // both have looked
+          ok = !shared || meet(&sh.both, n_both);  // both have looked
+          if (!ok) break;
           const unsigned flags = __ballot_sync(0xffffffffu, found && seen);
           if (lane == 0) sh.bad[k][warp & 3] = flags;
           if (found) {
@@ -845,11 +848,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           fence_proxy_async_smem();  // the zeros, to the product's reads
-          if (shared) {
-            both_sync();
-          } else {
-            item_any(k, false);
-          }
+          ok = shared ? meet(&sh.both, n_both) : meet(&sh.looked[k], n_looked);
+          if (!ok) break;
           unsigned bad[4];
 #pragma unroll
           for (int b = 0; b < 4; ++b) bad[b] = sh.bad[k][b];
