@@ -19,10 +19,10 @@
 // Bound, for chunks, by the chain of a step, which two items overlap only in part and TMEM has
 // no room for a third: scores 300 clocks behind the product, maximum 500, exponentials 1900
 // (the special-function unit alone takes 1024), the product's turn 1100.  2048 tokens behind
-// 6144, 32 heads of 128 over 8: 280 us, 860 TFLOP/s, 51 % of cuBLAS's burst rate; tensor pipe
+// 6144, 32 heads of 128 over 8: 281 us, 856 TFLOP/s, 51 % of cuBLAS's burst rate; tensor pipe
 // 38 %, special-function unit 47 %, issue slots 36 % of the time.  For decode by HBM between the
 // first loads (8 us, the search for the items ahead of them) and the last blocks and the join:
-// 64 requests of 3000 to 8191 keys take 273 us, 5.3 TB/s, 82 % of the copy rate.  (Bringing the
+// 64 requests of 3000 to 8191 keys take 270 us, 5.4 TB/s, 83 % of the copy rate.  (Bringing the
 // next block's first tiles to L2 while the last of this one's are worked on changed nothing.)
 //
 // P is rounded to the caches' 16-bit type because a product's two operands have one type and V
