@@ -850,6 +850,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           fence_proxy_async_smem();  // the zeros, to the product's reads
           ok = shared ? meet(&sh.both, n_both) : meet(&sh.looked[k], n_looked);
           if (!ok) break;
+          tmem_st_wait();  // O, if this step rescaled it: stores and loads are not ordered
           unsigned bad[4];
 #pragma unroll
           for (int b = 0; b < 4; ++b) bad[b] = sh.bad[k][b];
