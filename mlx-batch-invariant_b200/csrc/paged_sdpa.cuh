@@ -43,15 +43,17 @@ __device__ __forceinline__ float fold_value(float big, float x, float fa, float 
 }
 
 // The row's result from its joined (m, l): 1 / (l + sink's share), 0 for a row that sees
-// nothing.  `sink` is the head's extra logit in units of log 2.
+// nothing, whatever its sink (of -inf, -inf - -inf would be NaN).  `sink` is the head's extra
+// logit in units of log 2.
 __device__ __forceinline__ float row_scale(float m, float l, bool has_sink, float sink) {
+  if (l == 0.f) return 0.f;
   float f = 1.f;
   if (has_sink) {
     const float top = fmaxf(m, sink);
     f = m == top ? 1.f : exp2_approx(m - top);
     l = __fadd_rn(__fmul_rn(l, f), exp2_approx(sink - top));
   }
-  return l == 0.f ? 0.f : __fdiv_rn(f, l);
+  return __fdiv_rn(f, l);
 }
 // (+ 0.f: a result of -0 becomes +0, whether or not blocks that add nothing were visited)
 __device__ __forceinline__ float row_value(float o, float scale) {

@@ -1,5 +1,5 @@
 """paged_attention where several special values meet: non-finite values of keys in a step whose
-scores move the running maximum.
+scores move the running maximum, and sink logits that are infinite.
 
 Everything here is compared bit for bit with a call that lacks the special value, or element by
 element within the bound that test_paged_gpu.py derives."""
@@ -7,8 +7,9 @@ element within the bound that test_paged_gpu.py derives."""
 import pytest
 import torch
 
+import mlx_batch_invariant_b200 as bi
 from mlx_batch_invariant_b200 import _lib
-from test_paged_gpu import BF16, FP16, Batch, same_bits
+from test_paged_gpu import BF16, FP16, FP32, Batch, ints, randn, same_bits
 
 pytestmark = pytest.mark.gpu
 
@@ -75,3 +76,33 @@ def test_visible_values_where_the_maximum_moves(D, dtype):
         hit = torch.zeros_like(got, dtype=torch.bool)
         hit[first:q[0], 4:, 5] = True
         assert same_bits(got.masked_fill(hit, 0), want.masked_fill(hit, 0))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("sink", [-float("inf"), float("inf"), float("nan")])
+def test_rows_that_see_nothing_whatever_the_sink(dtype, sink):
+    """Zeros, as documented, where a row sees no key: whole and split over the grid."""
+    b = Batch([5, 3, 2, 40], [0, 0, 0, 9000], 8, 2, 64, 16, dtype)
+    b.lens = ints([2, 3, 0, 20])  # rows without a position: 3 of the first, 2, 20 of the last
+    got = b.run(sinks=torch.full((8,), sink, device="cuda"))
+    for lo, hi in ((0, 3), (8, 10), (10, 30)):
+        assert not got[lo:hi].any() and not got[lo:hi].isnan().any()
+    # a long request whose first tokens lie before its sequence, its keys split
+    s = Batch([300], [9000], 32, 8, 128 if dtype != FP32 else 64, 64, dtype, seed=6)
+    s.lens = ints([200])
+    got = s.run(sinks=torch.full((32,), sink, device="cuda"))
+    assert not got[:100].any() and not got[:100].isnan().any()
+    if sink == -float("inf"):
+        assert got[100:].isfinite().all() and got[100:].any(-1).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_a_sink_of_minus_infinity_is_none(dtype):
+    """e^-inf = 0: the bits of a call without sinks, next to heads that have one."""
+    b = Batch([1, 150, 9], [7000, 0, 800], 8, 2, 64, 32, dtype, seed=3)
+    none, sinks = b.run(), randn((8,), dtype, 4)
+    some = b.run(sinks=sinks)
+    off = sinks.clone()
+    off[::2] = -float("inf")
+    got = b.run(sinks=off)
+    assert same_bits(got[:, ::2], none[:, ::2]) and same_bits(got[:, 1::2], some[:, 1::2])
