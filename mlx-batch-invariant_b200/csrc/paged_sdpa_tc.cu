@@ -41,6 +41,7 @@
 // added to those rows' results by hand.
 #include <algorithm>
 
+#include "bounded_wait.h"
 #include "paged_sdpa.cuh"
 
 namespace bi {
@@ -129,25 +130,14 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
-// A whole warp's wait, bounded like mbar_wait; a loop of few instructions (the kernel's code
-// has to stay within the instruction cache: at 142 KB every step of it was fetched anew, and
-// the kernel ran no faster than its code came in).
+// A whole warp's wait, bounded like mbar_wait (the flag may be null); a loop of few instructions
+// (the kernel's code has to stay within the instruction cache: at 142 KB every step of it was
+// fetched anew, and the kernel ran no faster than its code came in).
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity,
                                           const volatile int* abort_flag) {
   const uint32_t addr = smem_u32(bar);
-  bool ok = true;
-  long long start = 0;
-#pragma unroll 1
-  for (uint32_t it = 0; !mbar_try_wait(addr, parity); ++it) {
-    if ((it & 255u) == 255u) {
-      const long long now = clock64();
-      if (start == 0) start = now;
-      if (*abort_flag || now - start > kWaitBudgetCycles) {
-        ok = false;
-        break;
-      }
-    }
-  }
+  const bool ok = bounded_wait([&] { return mbar_try_wait(addr, parity); },
+                               [] { return clock64(); }, abort_flag, kWaitBudgetCycles);
   return __all_sync(0xffffffffu, ok);
 }
 // One lane of the converged warp.
