@@ -56,6 +56,7 @@ constexpr int kTmemCols = 512;        // per item: S (P over its second half) an
 constexpr float kSlack = 8.f;         // log 2 of how far weights may exceed 1
 constexpr int kMaxStages = 12;
 constexpr int kBlockKeys = 1 << kTcShift;
+constexpr long long kCopyBudgetCycles = 20000000LL;  // about 10 ms
 
 enum : unsigned { kSiteProducer = 1, kSiteMma = 2, kSiteSoftmax = 3, kSiteDrain = 4 };
 
@@ -139,6 +140,12 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity,
   const bool ok = bounded_wait([&] { return mbar_try_wait(addr, parity); },
                                [] { return clock64(); }, abort_flag, kWaitBudgetCycles);
   return __all_sync(0xffffffffu, ok);
+}
+// The same for copies of a block that is giving up, with a limit of some milliseconds each.
+__device__ __forceinline__ void copy_wait(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  bounded_wait([&] { return mbar_try_wait(addr, parity); }, [] { return clock64(); }, nullptr,
+               kCopyBudgetCycles);
 }
 // One lane of the converged warp.
 __device__ __forceinline__ bool elect_one() {
@@ -339,6 +346,7 @@ struct Shared {
   uint32_t tmem;
   int abort_flag;
   int shared;             // the items share K and V
+  int loaded;             // K and V tiles that the producer has asked for
   Item item[2];
   int add[2];             // the item's next product is added to O (it does not start a key block)
   int hit[2];             // 1 + the last step whose V has such a value
@@ -447,8 +455,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto load = [&](const CUtensorMap* map, int k, int t0, int pg) {
         const int stage = n % C::kStages;
         ok = ok && warp_wait(&sh.empty[stage], ((n / C::kStages) & 1) ^ 1u, abort_flag);
-        ++n;
         if (!ok) return;
+        ++n;
         if (lane == 0) mbar_arrive_expect_tx(&sh.full[stage], C::kTileBytes);
         __syncwarp();
         if (side == k && sub < n_box) {
@@ -478,13 +486,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         pg0 = pg1;
         pg1 = pg2;
       }
-      if (!ok) {
-        if (lane == 0) {
-          *abort_flag = 1;
-          record_error(&g_error_word_tc, (kSiteProducer << 8) | kErrReasonTimeout);
-        }
-        sleep_ns(200000);  // the copies in flight land
+      if (!ok && lane == 0) {
+        *abort_flag = 1;
+        record_error(&g_error_word_tc, (kSiteProducer << 8) | kErrReasonTimeout);
       }
+      if (lane == 0) sh.loaded = n;
     } else if (warp == 9) {
       // ---------------- tcgen05.mma ----------------
       // The whole warp walks the steps, so that what it computes is uniform, and one lane
@@ -967,6 +973,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 9) {
     __syncwarp();
     tmem_dealloc(tmem, kTmemCols);
+  } else if (warp == 8 && __builtin_expect(*abort_flag, 0)) {
+    // Somebody gave up, so nobody has waited for the copies in flight: the block's shared memory
+    // is not given back while they may still write to it.
+    for (int k = 0; k < 2; ++k) {
+      if (sh.item[k].steps > 0) copy_wait(&sh.q_full[k], 0);
+    }
+    const int n = sh.loaded;
+    for (int i = max(0, n - C::kStages); i < n; ++i) {
+      copy_wait(&sh.full[i % C::kStages], (i / C::kStages) & 1);
+    }
   }
 }
 
