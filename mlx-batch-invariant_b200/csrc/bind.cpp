@@ -6,13 +6,16 @@
 // type, CUDA, the dtypes, shapes and strides that the kernels take as they are), allocates the
 // outputs and calls the C ABI: 6 to 9 us.  Whatever is not the plain case returns None, and the
 // Python function goes its full way, with its checks and messages; a status that is not 0 comes
-// back as a number for it to raise.
+// back as a number for it to raise.  No C++ exception leaves a function here: what torch throws
+// becomes the Python exception that torch makes of it (running out of memory among them).
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <exception>
 #include <optional>
 
 #include "bi.h"
@@ -27,11 +30,30 @@ decltype(&bi_paged_sdpa_workspace) g_workspace = nullptr;
 using at::ScalarType;
 using at::Tensor;
 
+// All that a plain CUDA tensor's keys may be.  Tensors under vmap, jvp, grad or functionalize,
+// nested ones and ones that only stand for zeros are of the exact tensor type too; they have a
+// key more, and no storage or not their values in it.
+constexpr c10::DispatchKeySet kPlainKeys =
+    c10::DispatchKeySet({c10::DispatchKey::CUDA, c10::DispatchKey::AutogradCUDA,
+                         c10::DispatchKey::AutocastCUDA, c10::DispatchKey::ADInplaceOrView});
+
 // The tensor of a plain CUDA tensor argument, else null.
 const Tensor* cuda_tensor(PyObject* o) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const Tensor& t = THPVariable_Unpack(o);
-  return t.defined() && t.is_cuda() && t.layout() == at::kStrided ? &t : nullptr;
+  return t.defined() && t.is_cuda() && (t.key_set() | kPlainKeys) == kPlainKeys && t.has_storage()
+             ? &t : nullptr;
+}
+
+// What F answers, or the Python exception of what it throws.
+template <PyObject* (*F)(PyObject* const*, Py_ssize_t)>
+PyObject* guarded(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  try {
+    return F(a, n);
+  } catch (...) {
+    torch::translate_exception_to_python(std::current_exception());
+    return nullptr;
+  }
 }
 
 bool is_vector(const Tensor* t, ScalarType type, int64_t n, c10::Device dev) {
@@ -87,7 +109,7 @@ void* stream_of(c10::Device dev) {
 }
 
 // (query_lens, context_lens, block_table, page_size, num_tokens, free_pages, free_head)
-PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
+PyObject* plan(PyObject* const* a, Py_ssize_t n) {
   if (n != 7 || g_plan == nullptr || !PyLong_CheckExact(a[3]) || !PyLong_CheckExact(a[4])) {
     Py_RETURN_NONE;
   }
@@ -115,38 +137,33 @@ PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
       Py_RETURN_NONE;
     }
   }
-  try {
-    const c10::cuda::CUDAGuard guard(dev);
-    const Tensor store = empty({16 * (tokens + 2) + 8 * R + 64}, at::kByte, dev);
-    int64_t at = 0;
-    Tensor pos = carve(store, at, tokens, at::kLong), slots = carve(store, at, tokens, at::kLong),
-           start = carve(store, at, R + 1, at::kInt), seq = carve(store, at, R, at::kInt), next;
-    if (alloc) next = carve(store, at, 1, at::kInt);
-    const int st = g_plan(
-        q->const_data_ptr<int>(), c->const_data_ptr<int>(), R, tokens,
-        table->mutable_data_ptr<int>(), table->stride(0), table->size(1), page,
-        alloc ? free->const_data_ptr<int>() : nullptr, alloc ? free->size(0) : 0,
-        alloc ? head->const_data_ptr<int>() : nullptr, start.mutable_data_ptr<int>(),
-        seq.mutable_data_ptr<int>(), pos.mutable_data_ptr<int64_t>(),
-        slots.mutable_data_ptr<int64_t>(), alloc ? next.mutable_data_ptr<int>() : nullptr,
-        stream_of(dev));
-    if (st != BI_OK) return PyLong_FromLong(st);
-    PyObject* out = PyTuple_New(5);
-    if (out == nullptr) return nullptr;
-    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(start)));
-    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(seq)));
-    PyTuple_SET_ITEM(out, 2, THPVariable_Wrap(std::move(pos)));
-    PyTuple_SET_ITEM(out, 3, THPVariable_Wrap(std::move(slots)));
-    PyTuple_SET_ITEM(out, 4, alloc ? THPVariable_Wrap(std::move(next)) : Py_NewRef(Py_None));
-    return out;
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+  const c10::cuda::CUDAGuard guard(dev);
+  const Tensor store = empty({16 * (tokens + 2) + 8 * R + 64}, at::kByte, dev);
+  int64_t at = 0;
+  Tensor pos = carve(store, at, tokens, at::kLong), slots = carve(store, at, tokens, at::kLong),
+         start = carve(store, at, R + 1, at::kInt), seq = carve(store, at, R, at::kInt), next;
+  if (alloc) next = carve(store, at, 1, at::kInt);
+  const int st = g_plan(
+      q->const_data_ptr<int>(), c->const_data_ptr<int>(), R, tokens,
+      table->mutable_data_ptr<int>(), table->stride(0), table->size(1), page,
+      alloc ? free->const_data_ptr<int>() : nullptr, alloc ? free->size(0) : 0,
+      alloc ? head->const_data_ptr<int>() : nullptr, start.mutable_data_ptr<int>(),
+      seq.mutable_data_ptr<int>(), pos.mutable_data_ptr<int64_t>(),
+      slots.mutable_data_ptr<int64_t>(), alloc ? next.mutable_data_ptr<int>() : nullptr,
+      stream_of(dev));
+  if (st != BI_OK) return PyLong_FromLong(st);
+  PyObject* out = PyTuple_New(5);
+  if (out == nullptr) return nullptr;
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(start)));
+  PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(seq)));
+  PyTuple_SET_ITEM(out, 2, THPVariable_Wrap(std::move(pos)));
+  PyTuple_SET_ITEM(out, 3, THPVariable_Wrap(std::move(slots)));
+  PyTuple_SET_ITEM(out, 4, alloc ? THPVariable_Wrap(std::move(next)) : Py_NewRef(Py_None));
+  return out;
 }
 
 // (qkv, cos, sin, positions, slots, k_cache, v_cache, out)
-PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+PyObject* rope(PyObject* const* a, Py_ssize_t n) {
   if (n != 8 || g_rope == nullptr) Py_RETURN_NONE;
   const Tensor *qkv = cuda_tensor(a[0]), *cs = cuda_tensor(a[1]), *sn = cuda_tensor(a[2]),
                *pos = cuda_tensor(a[3]), *slots = cuda_tensor(a[4]), *k = cuda_tensor(a[5]),
@@ -181,26 +198,21 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
       Py_RETURN_NONE;
     }
   }
-  try {
-    const c10::cuda::CUDAGuard guard(dev);
-    Tensor out = given != nullptr ? *given : empty({T, hq, hd}, type, dev);
-    const int st = g_rope(
-        qkv->const_data_ptr(), T > 1 ? qkv->stride(0) : width, T, hq, hk, hd, 2 * cs->size(1),
-        cs->const_data_ptr<float>(), sn->const_data_ptr<float>(), cs->size(0),
-        pos->const_data_ptr<int64_t>(), slots->const_data_ptr<int64_t>(), out.mutable_data_ptr(),
-        k->mutable_data_ptr(), ks, v->mutable_data_ptr(), vs, k->size(0), k->size(2), code,
-        stream_of(dev));
-    if (st != BI_OK) return PyLong_FromLong(st);
-    return given != nullptr ? Py_NewRef(a[7]) : THPVariable_Wrap(std::move(out));
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+  const c10::cuda::CUDAGuard guard(dev);
+  Tensor out = given != nullptr ? *given : empty({T, hq, hd}, type, dev);
+  const int st = g_rope(
+      qkv->const_data_ptr(), T > 1 ? qkv->stride(0) : width, T, hq, hk, hd, 2 * cs->size(1),
+      cs->const_data_ptr<float>(), sn->const_data_ptr<float>(), cs->size(0),
+      pos->const_data_ptr<int64_t>(), slots->const_data_ptr<int64_t>(), out.mutable_data_ptr(),
+      k->mutable_data_ptr(), ks, v->mutable_data_ptr(), vs, k->size(0), k->size(2), code,
+      stream_of(dev));
+  if (st != BI_OK) return PyLong_FromLong(st);
+  return given != nullptr ? Py_NewRef(a[7]) : THPVariable_Wrap(std::move(out));
 }
 
 // (q, k_cache, v_cache, block_table, query_start, seq_lens, scale, window, first_tokens, sinks,
 //  out)
-PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+PyObject* attention(PyObject* const* a, Py_ssize_t n) {
   if (n != 11 || g_sdpa == nullptr || !PyLong_CheckExact(a[8])) Py_RETURN_NONE;
   const Tensor *q = cuda_tensor(a[0]), *k = cuda_tensor(a[1]), *v = cuda_tensor(a[2]),
                *table = cuda_tensor(a[3]), *start = cuda_tensor(a[4]), *seq = cuda_tensor(a[5]);
@@ -261,29 +273,24 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       Py_RETURN_NONE;
     }
   }
-  try {
-    const c10::cuda::CUDAGuard guard(dev);
-    Tensor out = given != nullptr ? *given : empty({T, H, D}, type, dev);
-    const int64_t os[2] = {out.stride(0), out.stride(1)};
-    const int64_t bytes = g_workspace(T, R, H, D, table->size(1), k->size(2));
-    const Tensor ws = empty({bytes}, at::kByte, dev);
-    const int st = g_sdpa(
-        q->const_data_ptr(), qs, k->const_data_ptr(), ks, v->const_data_ptr(), vs, k->size(0),
-        k->size(2), table->const_data_ptr<int>(), table->stride(0), table->size(1),
-        start->const_data_ptr<int>(), seq->const_data_ptr<int>(),
-        sinks != nullptr ? sinks->const_data_ptr() : nullptr, static_cast<float>(scale), window,
-        first, T, R, H, Hkv, D, code, out.mutable_data_ptr(), os, ws.mutable_data_ptr(), bytes,
-        stream_of(dev));
-    if (st != BI_OK) return PyLong_FromLong(st);
-    return given != nullptr ? Py_NewRef(a[10]) : THPVariable_Wrap(std::move(out));
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+  const c10::cuda::CUDAGuard guard(dev);
+  Tensor out = given != nullptr ? *given : empty({T, H, D}, type, dev);
+  const int64_t os[2] = {out.stride(0), out.stride(1)};
+  const int64_t bytes = g_workspace(T, R, H, D, table->size(1), k->size(2));
+  const Tensor ws = empty({bytes}, at::kByte, dev);
+  const int st = g_sdpa(
+      q->const_data_ptr(), qs, k->const_data_ptr(), ks, v->const_data_ptr(), vs, k->size(0),
+      k->size(2), table->const_data_ptr<int>(), table->stride(0), table->size(1),
+      start->const_data_ptr<int>(), seq->const_data_ptr<int>(),
+      sinks != nullptr ? sinks->const_data_ptr() : nullptr, static_cast<float>(scale), window,
+      first, T, R, H, Hkv, D, code, out.mutable_data_ptr(), os, ws.mutable_data_ptr(), bytes,
+      stream_of(dev));
+  if (st != BI_OK) return PyLong_FromLong(st);
+  return given != nullptr ? Py_NewRef(a[10]) : THPVariable_Wrap(std::move(out));
 }
 
 // Addresses of libbi.so's functions, in the order of the pointers above.
-PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
+PyObject* init(PyObject* const* a, Py_ssize_t n) {
   if (n != 4) {
     PyErr_SetString(PyExc_TypeError, "init takes the four entry points' addresses");
     return nullptr;
@@ -300,7 +307,8 @@ PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
-#define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f)), METH_FASTCALL
+#define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&guarded<f>)), \
+                METH_FASTCALL
 PyMethodDef g_methods[] = {{"init", FAST(init), nullptr},
                            {"plan", FAST(plan), nullptr},
                            {"rope", FAST(rope), nullptr},
