@@ -319,4 +319,11 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_bind",
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__bind(void) { return PyModule_Create(&g_module); }
+PyMODINIT_FUNC PyInit__bind(void) {
+  PyObject* m = PyModule_Create(&g_module);
+  // the torch whose headers this was compiled with; with another one it is not used
+  if (m != nullptr && PyModule_AddStringConstant(m, "torch_version", BI_TORCH_VERSION) != 0) {
+    Py_CLEAR(m);
+  }
+  return m;
+}

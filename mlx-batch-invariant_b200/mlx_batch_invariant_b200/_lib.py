@@ -7,6 +7,7 @@ fallback: if it is missing or the device is not an sm_100 GPU, every operator ra
 import ctypes
 import os
 import threading
+import warnings
 
 import torch
 
@@ -130,19 +131,39 @@ def lib():
     return _lib
 
 
+class FullWay:
+    """Stands for the _bind module where there is none: takes no call, so that each goes through
+    the checks in _paged.py and ctypes."""
+
+    @staticmethod
+    def plan(*args):
+        return None
+
+    rope = attention = plan
+
+
 def short_way():
-    """The _bind module, the short way to the paged-cache operators, set to this libbi.so."""
+    """The _bind module, the short way to the paged-cache operators, set to this libbi.so; where
+    it cannot be used, FullWay, with a warning."""
     global _short
     if _short is None:
         handle = lib()
         try:
             from . import _bind as module
+            built_for = getattr(module, "torch_version", "an unknown version")
+            why = ("it was built for torch %s, this is %s" % (built_for, torch.__version__)
+                   if built_for != torch.__version__ else None)
         except ImportError as e:
-            raise RuntimeError("_bind.so is not built (%s); run python "
-                               "mlx-batch-invariant_b200/build.py" % e)
-        module.init(*[ctypes.cast(getattr(handle, name), _vp).value for name in (
-            "bi_paged_plan", "bi_rope_kv_paged", "bi_paged_sdpa", "bi_paged_sdpa_workspace")])
-        _short = module
+            why = e
+        if why is None:
+            module.init(*[ctypes.cast(getattr(handle, name), _vp).value for name in (
+                "bi_paged_plan", "bi_rope_kv_paged", "bi_paged_sdpa", "bi_paged_sdpa_workspace")])
+            _short = module
+        else:
+            warnings.warn("the paged operators are called through ctypes, which takes the host "
+                          "some 20 us longer: _bind cannot be used (%s); run python "
+                          "mlx-batch-invariant_b200/build.py" % why, RuntimeWarning, stacklevel=3)
+            _short = FullWay
     return _short
 
 
