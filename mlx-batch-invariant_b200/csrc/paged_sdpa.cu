@@ -24,6 +24,8 @@ constexpr int kSimtThreads = 32 * kSimtWarps;
 constexpr int kSimtRows = 4;  // per warp
 constexpr int kSimtTile = kSimtWarps * kSimtRows;
 constexpr int kSimtKeys = 32;  // of a step
+// Its partial results are one a key block, as those of tiles of few rows are (entries_of).
+static_assert(kSimtTile <= kFineRows, "a CUDA-core tile counts as one of few rows");
 
 template <int DC>
 struct SimtCfg {
@@ -627,7 +629,7 @@ int launch_paged_sdpa(const PagedSdpaArgs& a, cudaStream_t stream) {
 
   // tiles of all requests: at most one ragged tile each
   const int64_t tiles = a.T / p.tile_tok + std::min(a.R, a.T);
-  p.fine_rows = 16;
+  p.fine_rows = kFineRows;
   // few tiles: one piece for every place is enough; many: finer, to even out ragged lengths
   p.finer = tiles * p.groups >= p.target ? 4 : 1;
   // (the spans are rounded in fp32: a little above finer x target pieces)

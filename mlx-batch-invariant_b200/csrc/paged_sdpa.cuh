@@ -20,6 +20,7 @@ namespace bi {
 namespace psdpa {
 
 constexpr int kTcShift = 9, kSimtShift = 7;  // log 2 of the keys of a block on either route
+constexpr int kFineRows = 16;  // tiles of at most so many rows are cheap to split (is_few)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr unsigned kErrReasonRange = 2;
 
