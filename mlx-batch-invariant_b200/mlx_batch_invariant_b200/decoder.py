@@ -494,8 +494,11 @@ class PagedDecodeGraph:
         """tokens: per request the token to go on from, or None for one that does not run."""
         if len(tokens) != self.server.requests:
             raise ValueError("%d entries for %d requests" % (len(tokens), self.server.requests))
+        ids, vocab = [0 if t is None else int(t) for t in tokens], self.server.model.cfg.vocab
+        if any(not 0 <= t < vocab for t in ids):
+            raise ValueError("token ids must be in [0, %d)" % vocab)
         self._active = [int(t is not None) for t in tokens]
-        self.tok.copy_(torch.tensor([0 if t is None else int(t) for t in tokens]))
+        self.tok.copy_(torch.tensor(ids))
         self.running.copy_(torch.tensor(self._active, dtype=torch.int32))
 
     def step(self):
