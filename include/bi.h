@@ -368,8 +368,8 @@ int64_t bi_paged_sdpa_workspace(int64_t T, int64_t R, int64_t H, int64_t D, int6
  *           `out` outside every request are left as they were.
  *   k, v    (n_pages, Hkv, page_size, D), strides of page, head and token.
  *   sinks   nullable (H,) in the q dtype: one extra logit per head.
- * All 16-byte aligned with strides that are multiples of 16 bytes.  H % Hkv == 0; D a multiple
- * of 32 up to 256; scale finite and >= 0.  A row that sees no key
+ * All 16-byte aligned with positive strides that are multiples of 16 bytes (of out's dimensions
+ * of one any multiple).  H % Hkv == 0; D a multiple of 32 up to 256; scale finite and >= 0.  A row that sees no key
  * returns zeros.  Keys that a row does not see do not reach it, whatever they hold.  A page
  * number outside [0, n_pages) reads as zeros.  query_start and seq_lens are clamped to T and
  * to what a row of the table holds.

@@ -269,6 +269,7 @@ PyObject* attention(PyObject* const* a, Py_ssize_t n) {
     if (given == nullptr || given->scalar_type() != type || given->device() != dev ||
         given->sizes() != q->sizes() || given->stride(2) != 1 ||
         given->stride(0) % vec != 0 || given->stride(1) % vec != 0 ||
+        (T > 1 && given->stride(0) == 0) || (H > 1 && given->stride(1) == 0) ||
         !aligned16(given->const_data_ptr())) {
       Py_RETURN_NONE;
     }

@@ -704,7 +704,8 @@ int bi_paged_sdpa(const void* q, const int64_t q_strides[2], const void* k,
          v_strides[i] % vec == 0;
   }
   ok = ok && q_strides[0] > 0 && q_strides[1] > 0 && aligned16(out) &&
-       out_strides[0] % vec == 0 && out_strides[1] % vec == 0;
+       out_strides[0] % vec == 0 && out_strides[1] % vec == 0 &&
+       (T == 1 || out_strides[0] > 0) && (H == 1 || out_strides[1] > 0);
   if (!ok) {
     return set_error(BI_ERR_MISALIGNED, "q, out and the caches must be 16-byte aligned with "
                      "positive strides that are multiples of 16 bytes");

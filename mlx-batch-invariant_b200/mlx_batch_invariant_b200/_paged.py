@@ -247,8 +247,8 @@ def paged_attention(q, k_cache, v_cache, block_table, query_start, seq_lens, *, 
     ``first_tokens`` first ones.  ``sinks`` is an optional logit per query head, as in
     scaled_dot_product_attention.  Heads are grouped: heads % kv_heads == 0.
 
-    Rows outside every request are not written: pass ``out`` (which may be ``q``) where that
-    matters.  A row that sees nothing returns zeros.  Lengths are device data; they are clamped
+    Rows outside every request are not written: pass ``out`` (which may be ``q``, not an expanded
+    tensor) where that matters.  A row that sees nothing returns zeros.  Lengths are device data; they are clamped
     to ``q`` and to the table, and pages outside the cache read as zeros.
     """
     compiling = torch.compiler.is_compiling()
@@ -297,6 +297,8 @@ def paged_attention(q, k_cache, v_cache, block_table, query_start, seq_lens, *, 
                             or (D > 1 and out.stride(2) != 1)):
         raise ValueError("out must be %s %s with a contiguous last dimension"
                          % (tuple(q.shape), q.dtype))
+    if out is not None and any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+        raise ValueError("out must not be an expanded tensor")
     if not compiling:
         _check_aligned(k_cache, v_cache)
     dev = _check_cuda(q, k_cache, v_cache, block_table, query_start, seq_lens, sinks, out)
