@@ -715,8 +715,6 @@ int bi_paged_sdpa(const void* q, const int64_t q_strides[2], const void* k,
     return set_error(BI_ERR_INVALID, "workspace is null, misaligned or smaller than "
                      "bi_paged_sdpa_workspace of no tokens");
   }
-  int st = check_device();
-  if (st) return st;
   PagedSdpaArgs a;
   a.q = q;
   a.k = k;
@@ -749,6 +747,11 @@ int bi_paged_sdpa(const void* q, const int64_t q_strides[2], const void* k,
   a.dtype = dtype;
   a.workspace = workspace;
   a.workspace_bytes = workspace_bytes;
+  if (!paged_sdpa_fits(a)) {
+    return set_error(BI_ERR_UNSUPPORTED, "more than 2^30 requests or tiles of query rows");
+  }
+  const int st = check_device();
+  if (st) return st;
   return launch_paged_sdpa(a, static_cast<cudaStream_t>(stream));
 }
 

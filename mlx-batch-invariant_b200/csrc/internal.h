@@ -157,6 +157,8 @@ struct PagedSdpaArgs {
 };
 int64_t paged_sdpa_workspace(int64_t T, int64_t R, int64_t H, int64_t D, int64_t width,
                              int64_t page);
+// Are the call's items few enough to be counted on the device?
+bool paged_sdpa_fits(const PagedSdpaArgs& a);
 int launch_paged_sdpa(const PagedSdpaArgs& a, cudaStream_t stream);
 
 int launch_gemm_tc(const GemmArgs& g, cudaStream_t stream);

@@ -571,10 +571,32 @@ int64_t paged_sdpa_workspace(int64_t T, int64_t R, int64_t H, int64_t D, int64_t
   return psdpa::info_bytes(R) + part;
 }
 
+namespace psdpa {
+// How the heads and tokens of a call make tiles of `rows` rows.
+struct Tiling {
+  int64_t group_heads, subs, tile_tok;  // heads of a group, groups of a KV head, tokens of a tile
+  int64_t tiles;                        // of all requests: at most one ragged tile each
+  explicit Tiling(const PagedSdpaArgs& a) {
+    const int64_t rows = paged_tc_takes(a) ? 128 : kSimtTile, G = a.H / a.Hkv;
+    group_heads = std::min(G, rows);
+    subs = (G + rows - 1) / rows;
+    tile_tok = rows / group_heads;
+    tiles = a.T / tile_tok + std::min(a.R, a.T);
+  }
+};
+}  // namespace psdpa
+
+bool paged_sdpa_fits(const PagedSdpaArgs& a) {
+  const psdpa::Tiling t(a);
+  // items are counted in 32 bits that stop at kMuch; the splits of the keys add less than 2^16
+  const int64_t most = static_cast<int64_t>(psdpa::kMuch) - (1 << 16);
+  return a.R <= most && t.tiles <= most / (a.Hkv * t.subs);
+}
+
 int launch_paged_sdpa(const PagedSdpaArgs& a, cudaStream_t stream) {
   using namespace psdpa;
   const bool tc = paged_tc_takes(a);
-  const int rows = tc ? 128 : kSimtTile;
+  const Tiling tiling(a);
   Params p;
   p.q = a.q;
   p.k = a.k;
@@ -608,14 +630,13 @@ int launch_paged_sdpa(const PagedSdpaArgs& a, cudaStream_t stream) {
   p.shift = tc ? kTcShift : kSimtShift;
   p.max_seq = static_cast<int>(
       std::min<int64_t>(a.width * a.page, INT32_MAX - (1 << kTcShift)));
-  p.group_heads = std::min(p.G, rows);
-  p.tile_tok = rows / p.group_heads;
-  const int subs = (p.G + rows - 1) / rows;
-  p.groups = p.Hkv * subs;
+  p.group_heads = static_cast<int>(tiling.group_heads);
+  p.tile_tok = static_cast<int>(tiling.tile_tok);
+  p.groups = static_cast<int>(a.Hkv * tiling.subs);
   p.by_tile = divider(p.tile_tok);
   p.by_page = divider(a.page);
   p.by_head = divider(p.group_heads);
-  p.by_group = divider(subs);
+  p.by_group = divider(tiling.subs);
   p.target = 2 * device_sm_count();
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   p.head = reinterpret_cast<int4*>(ws);
@@ -627,14 +648,12 @@ int launch_paged_sdpa(const PagedSdpaArgs& a, cudaStream_t stream) {
   p.part_o = reinterpret_cast<float*>(ws + info_bytes(a.R));
   p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<int64_t>(p.slots) * a.D);
 
-  // tiles of all requests: at most one ragged tile each
-  const int64_t tiles = a.T / p.tile_tok + std::min(a.R, a.T);
+  const int64_t tiles = tiling.tiles;
   p.fine_rows = kFineRows;
   // few tiles: one piece for every place is enough; many: finer, to even out ragged lengths
   p.finer = tiles * p.groups >= p.target ? 4 : 1;
   // (the spans are rounded in fp32: a little above finer x target pieces)
   const int64_t items = tiles * p.groups + static_cast<int64_t>(p.finer) * p.target + 64;
-  if (items > INT32_MAX) return set_error(BI_ERR_UNSUPPORTED, "too many query tiles");
   if (a.R > kFewRequests) {
     const int st = cuda_status(launch_early(schedule_kernel, 1u, kScheduleThreads, 0, stream, p),
                                "paged_sdpa schedule launch");
