@@ -191,8 +191,8 @@ def rope_kv_paged(qkv, cos, sin, positions, slots, k_cache, v_cache, *, out=None
     _check_caches(k_cache, v_cache, qkv.dtype)
     T, width = qkv.shape
     n_pages, hk, page, hd = k_cache.shape
-    if hd % 2:
-        raise ValueError("head_dim must be even, got %d" % hd)
+    if hd % 2 or hd == 0:
+        raise ValueError("head_dim must be even and positive, got %d" % hd)
     if width % hd or width // hd < 2 * hk:
         raise ValueError("a row of qkv has %d elements: not q heads and 2 x %d kv heads of %d"
                          % (width, hk, hd))
