@@ -353,8 +353,10 @@ int bi_rope_kv_paged(const void* qkv, int64_t qkv_stride, int64_t T, int64_t hq,
                      const int64_t v_strides[3], int64_t n_pages, int64_t page_size, int dtype,
                      void* stream);
 
-/* Bytes of workspace that bi_paged_sdpa makes full use of (of T = 0: the least it takes;
- * with less than the full amount long requests are split over fewer blocks, same bits). */
+/* Bytes of workspace that bi_paged_sdpa makes full use of, at most 256 MiB and the notes of R
+ * requests (of T = 0: the least it takes; with less than the full amount long requests, the later
+ * ones of the batch first, are not split, same bits).  It does not know the route: the tensor
+ * cores use a quarter of it. */
 int64_t bi_paged_sdpa_workspace(int64_t T, int64_t R, int64_t H, int64_t D, int64_t width,
                                 int64_t page_size);
 
@@ -369,9 +371,9 @@ int64_t bi_paged_sdpa_workspace(int64_t T, int64_t R, int64_t H, int64_t D, int6
  *   k, v    (n_pages, Hkv, page_size, D), strides of page, head and token.
  *   sinks   nullable (H,) in the q dtype: one extra logit per head.
  * All 16-byte aligned with positive strides that are multiples of 16 bytes (of out's dimensions
- * of one any multiple).  H % Hkv == 0; D a multiple of 32 up to 256; scale finite and >= 0.  A row that sees no key
- * returns zeros.  Keys that a row does not see do not reach it, whatever they hold.  A page
- * number outside [0, n_pages) reads as zeros.  query_start and seq_lens are clamped to T and
+ * of one any multiple).  H % Hkv == 0; D a multiple of 32 up to 256; scale finite and >= 0.
+ * A row that sees no key returns zeros, whatever its sink; a sink of -inf is none.  Keys that a
+ * row does not see do not reach it, whatever they hold.  A page number outside [0, n_pages) reads as zeros.  query_start and seq_lens are clamped to T and
  * to what a row of the table holds.
  * Invariance: a row's bits depend on its q, its keys and values, (dtype, D, H / Hkv,
  * page_size), scale, window, first_tokens and sinks alone -- not on the batch, on how many

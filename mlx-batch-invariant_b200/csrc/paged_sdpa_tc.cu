@@ -18,12 +18,16 @@
 //
 // Bound, for chunks, by the chain of a step, which two items overlap only in part and TMEM has
 // no room for a third: scores 300 clocks behind the product, maximum 500, exponentials 1900
-// (the special-function unit alone takes 1024), the product's turn 1100.  2048 tokens behind
-// 6144, 32 heads of 128 over 8: 281 us, 856 TFLOP/s, 51 % of cuBLAS's burst rate; tensor pipe
-// 38 %, special-function unit 47 %, issue slots 36 % of the time.  For decode by HBM between the
-// first loads (8 us, the search for the items ahead of them) and the last blocks and the join:
-// 64 requests of 3000 to 8191 keys take 270 us, 5.4 TB/s, 83 % of the copy rate.  (Bringing the
-// next block's first tiles to L2 while the last of this one's are worked on changed nothing.)
+// (the special-function unit alone takes 1024), the product's turn 1100; and by waves that are
+// not full.  2048 tokens behind 6144, 32 heads of 128 over 8: 278 us in a graph (291 called from
+// Python), 864 TFLOP/s, 52 % of cuBLAS's burst rate; tensor pipe 38 %, special-function unit
+// 47 %, issue slots 36 % of the time.  Its 256 pairs of items make 1.73 waves on 148 SMs, which
+// alone is 13 %.  For decode by HBM between the first loads (8 us, the search for the items ahead
+// of them) and the last blocks and the join: 64 requests of 3000 to 8191 keys take 274 us in a
+// graph (307 called), 5.3 TB/s, 82 % of the copy rate.  (Bringing the next block's first tiles to
+// L2 while the last of this one's are worked on changed nothing.)  The softmax keeps a row's
+// running result and half its scores in registers; at D = 128 that spills (148 bytes stored, 204
+// loaded a thread), at D = 64 hardly (8 and 52).
 //
 // P is rounded to the caches' 16-bit type because a product's two operands have one type and V
 // has that one; the row's sum adds the weights before that rounding.  It adds half a step of the

@@ -73,6 +73,9 @@ def paged_plan(query_lens, context_lens, block_table, page_size, num_tokens, *, 
     negative or exceeds the table's row makes its request bring no tokens, a token without a
     page gets slot -1, and both, like more tokens than ``num_tokens``, are reported by
     ``_lib.device_error()``.
+
+    The outputs may share one allocation: a server that keeps ``next_head`` from step to step
+    keeps that step's positions and slots as well until the next one replaces it.
     """
     compiling = torch.compiler.is_compiling()
     if not compiling:
@@ -243,9 +246,12 @@ def paged_attention(q, k_cache, v_cache, block_table, query_start, seq_lens, *, 
     ``q`` (tokens, heads, head_dim) holds the requests' tokens one after the other: request
     r's are rows ``query_start[r]`` to ``query_start[r + 1]`` and are the last ones of its
     ``seq_lens[r]`` (whose keys and values are in the caches already).  A token at position p
-    sees the keys i <= p; with a ``window`` only those with i > p - window, and the sequence's
-    ``first_tokens`` first ones.  ``sinks`` is an optional logit per query head, as in
-    scaled_dot_product_attention.  Heads are grouped: heads % kv_heads == 0.
+    sees the keys i <= p; with a ``window`` (None or 0: without) only those with i > p - window,
+    and the sequence's ``first_tokens`` first ones.  ``sinks`` is an optional logit per query
+    head, as in scaled_dot_product_attention; -inf is none.  Heads are grouped: heads % kv_heads
+    == 0.  float16 / bfloat16 with head dim 64 or 128 and pages that divide or are multiples of
+    128 run on the tensor cores, with the weights rounded to that type ahead of the product with
+    v (scaled_dot_product_attention keeps them in fp32); everything else in fp32 throughout.
 
     Rows outside every request are not written: pass ``out`` (which may be ``q``, not an expanded
     tensor) where that matters.  A row that sees nothing returns zeros.  Lengths are device data; they are clamped
